@@ -92,6 +92,16 @@ SIGNATURES = {
     "hn_upsample_flatten": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "hn_lstm_layer": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "hn_linear_head": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "hn_gated_recurrence_states": (_sz, [_i64, _i64, _i64]),
+    "hn_gated_recurrence_workspace": (_sz, [_i64, _i64, _i64]),
+    "hn_gated_recurrence": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
+    "hn_gated_recurrence_bwd": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                     _i64, _i64, _i64, _i, _i, _vp]),
+    "hn_gated_recurrence_step": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i, _vp]),
+    "hn_gated_linear_workspace": (_sz, [_i64, _i64, _i64, _i, _i]),
+    "hn_gated_linear": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
+    "hn_gated_linear_bwd": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
+    "hn_dropout": (_i, [_vp, _vp, _vp, _i64, _i, _f, _c.c_uint64, _vp, _vp]),
 }
 
 _lib = None

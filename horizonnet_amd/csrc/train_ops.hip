@@ -4,6 +4,7 @@
 // per-step LSTM gate adjoint.  All HBM-bound, NHWC / row-major float32, float4 vectorised; column
 // reductions accumulate per-thread partials in f32 and combine across workgroups with f64 atomics.
 #include "hn_common.h"
+#include "seq_common.h"
 
 namespace {
 
@@ -859,19 +860,14 @@ __global__ __launch_bounds__(256) void upsample_flatten_bwd_kernel(const float* 
     }
 }
 
-// counter-based dropout mask: keep iff hash(seed, index) >= p * 2^32; out = in * keep / (1 - p)
-__device__ __forceinline__ unsigned hash32(unsigned long long x)
-{
-    x ^= x >> 33; x *= 0xff51afd7ed558ccdULL; x ^= x >> 33; x *= 0xc4ceb9fe1a85ec53ULL; x ^= x >> 33;
-    return (unsigned)x;
-}
+// counter-based dropout mask: keep iff the generator's bits at (seed, index) >= p * 2^32; out = in * keep / (1 - p)
 __global__ __launch_bounds__(256) void dropout_kernel(const float* __restrict__ in, float* __restrict__ out, long n, float p,
                                                       unsigned long long seed)
 {
     const unsigned thr = (unsigned)((double)p * 4294967296.0);
     const float sc = 1.0f / (1.0f - p);
     for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x)
-        out[i] = hash32(seed * 0x9e3779b97f4a7c15ULL + (unsigned long long)i) >= thr ? in[i] * sc : 0.f;
+        out[i] = seq_dropout_bits(seed * SEQ_DROPOUT_STRIDE, (unsigned long long)i) >= thr ? in[i] * sc : 0.f;
 }
 
 // Linear head adjoint: dlin[t*B+b][12] gathered from dbon / dcor; dy[row][k] = sum_o dlin[row][o] * w[o][k]

@@ -423,6 +423,47 @@ int hn_lstm_layer(const float* gx, const float* whh_fwd, const float* whh_rev, f
 int hn_linear_head(const float* y, const float* w, const float* bias, float* bon, float* cor,
                    int T, int B, void* stream);
 
+/* ---- sequence operators: the pieces of a recurrent block over the [T][B][C] sequence that hn_upsample_flatten builds and the LSTM layers
+ * read.  dtype: 0 float32, 1 bf16 (every tensor below that is `void*`; `float*` ones are float32 always).  Strides count elements. ---- */
+
+/* Gated linear recurrence, every channel by itself:  a = s(f), h_t = a_t h_{t-1} + (1 - a_t) v_t, y_t = s(o_t) h_t  (s: logistic function).
+ * f, v, o [T][B][C] by their time and sequence strides, channels contiguous; o may be null (y = h).  direction: 0 from the first step,
+ * 1 from the last, 2 the first C / 2 channels from the first step and the others from the last (the layout of hn_lstm_layer's y).
+ * h0 [B][C] or null (zeros); lengths [B] int32 (device) or null: a sequence's steps at or past its length are not read, y is 0 there and the
+ * state passes (values outside 0 .. T count as the nearest).  y [T][B][C], h_last [B][C] = the state behind the last step taken.
+ * states: hn_gated_recurrence_states() floats for hn_gated_recurrence_bwd, or null; workspace: hn_gated_recurrence_workspace() floats. */
+size_t hn_gated_recurrence_states(int64_t T, int64_t B, int64_t C);
+size_t hn_gated_recurrence_workspace(int64_t T, int64_t B, int64_t C);
+int hn_gated_recurrence(const void* f, int64_t f_t, int64_t f_b, const void* v, int64_t v_t, int64_t v_b, const void* o, int64_t o_t,
+                        int64_t o_b, const float* h0, const int* lengths, void* y, float* h_last, float* states, float* workspace,
+                        size_t workspace_floats, int64_t T, int64_t B, int64_t C, int dtype, int direction, void* stream);
+/* Its adjoint: dy [T][B][C] by strides, dh_last [B][C] or null; df, dv, d_o (iff o) [T][B][C] contiguous, 0 at and past a sequence's length;
+ * dh0 [B][C] or null; states as the forward call wrote them. */
+int hn_gated_recurrence_bwd(const void* f, int64_t f_t, int64_t f_b, const void* v, int64_t v_t, int64_t v_b, const void* o, int64_t o_t,
+                            int64_t o_b, const void* dy, int64_t dy_t, int64_t dy_b, const float* dh_last, const int* lengths,
+                            const float* states, void* df, void* dv, void* d_o, float* dh0, float* workspace, size_t workspace_floats,
+                            int64_t T, int64_t B, int64_t C, int dtype, int direction, void* stream);
+/* One step of B sequences: state [B][C] is updated in place, y [B][C]. */
+int hn_gated_recurrence_step(const void* f, int64_t f_b, const void* v, int64_t v_b, const void* o, int64_t o_b, float* state, void* y,
+                             int64_t B, int64_t C, int dtype, void* stream);
+
+/* Gated linear block:  y = act(x w_gate^T + b_gate) * (x w_up^T + b_up),  x [M][K], w [F][K] by their row strides, biases [F] or null,
+ * y [M][F] contiguous.  act: 0 silu, 1 gelu (error function), 2 sigmoid, 3 relu.  workspace: hn_gated_linear_workspace() bytes.
+ * hn_gated_linear_bwd: dy [M][F] by its row stride; dx [M][K], dw_* [F][K], db_* [F] contiguous, each may be null. */
+size_t hn_gated_linear_workspace(int64_t M, int64_t K, int64_t F, int dtype, int backward);
+int hn_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,
+                    const void* b_up, void* y, void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act,
+                    void* stream);
+int hn_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,
+                        const void* b_up, const void* dy, int64_t ld_dy, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
+                        void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act, void* stream);
+
+/* Dropout:  y[i] = residual[i] + (keep(i) ? x[i] / (1 - p) : 0), keep(i) = the generator's 32 bits at (seed, i) >= p 2^32: the generator of
+ * the training step (hn_train_forward's mask behind LSTM layer l is that of seed' = 2 seed + 1 + l).  residual may be null; seed_dev, if not
+ * null, is a device pointer to the 64-bit seed, read by the kernel.  y overlaps neither x nor
+ * residual.  The gradient of x is the same call on dy. */
+int hn_dropout(const void* x, const void* residual, void* y, int64_t n, int dtype, float p, uint64_t seed, const void* seed_dev, void* stream);
+
 /* Data gradient of hn_conv2d_nhwc (adjoint w.r.t. x): dz [B][Ho][Wo][Cout] -> dx [B][Hx][Wx][Cin] (+ add).
  * w_oihw: the ORIGINAL OIHW weights; w_scratch: Cout*Cin*KH*KW + 8192 floats of device scratch. */
 int hn_conv2d_dgrad_nhwc(const float* dz, const float* w_oihw, const float* add, float* dx, float* w_scratch, int B,

@@ -1,0 +1,568 @@
+"""Sequence operators on the device against the 64-bit oracle, whose bounds come from running error analysis (oracle/sequence_ref.py): a
+result may be off by what float32 arithmetic can add and by half a step of the type that it is stored in."""
+import pytest
+import torch
+
+import horizonnet_amd as hn
+from oracle import sequence_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+# a gate in bf16 mode uses the short exponential, whose error is |argument| units: arguments here stay below 8 in the mean, 12 at most
+EPS = {"f32": 16 * ref.U, "bf16": 40 * ref.U}
+
+
+def _normal(g, *shape, dtype=torch.float32, scale=1.0, mean=0.0):
+    return (torch.randn(*shape, generator=g) * scale + mean).to(dtype)
+
+
+def _near(name, got, want, off):
+    """|got - want| <= off + half a step of got's type at |want| + off, everywhere."""
+    assert got.shape == want.shape, name
+    half = ref.rounding(got.dtype)
+    got = got.detach().cpu().double()
+    room = off + half * (want.abs() + off) + 1e-30
+    bad = ~((got - want).abs() <= room)
+    assert not bool(bad.any()), "%s: %d of %d off; worst %.3g of its room %.3g (value %.4g)" % (
+        (name, int(bad.sum()), bad.numel()) + tuple(float(t.reshape(-1)[((got - want).abs() / room).nan_to_num(float("inf")).argmax()]) for t in
+                                                    ((got - want).abs(), room, want)))
+
+
+def _rec_case(T, B, C, dtype, gate=True, h0=True, lengths=None, seed=0):
+    g = torch.Generator().manual_seed(seed + 7 * T + 13 * B + C)
+    f = _normal(g, T, B, C, dtype=dtype, scale=1.5, mean=1.0)
+    v, dy = _normal(g, T, B, C, dtype=dtype), _normal(g, T, B, C, dtype=dtype)
+    o = _normal(g, T, B, C, dtype=dtype) if gate else None
+    h = _normal(g, B, C) if h0 else None
+    return f, v, o, h, dy, _normal(g, B, C), lengths
+
+
+def _rec_check(case, direction, name, place=lambda t: t.to(DEV)):
+    f, v, o, h, dy, dlast, lengths = case
+    want, off = ref.recurrence(f, v, o, h, lengths, direction, dy, dlast, EPS[name])
+    put = lambda t: None if t is None else place(t).detach().requires_grad_(True)  # noqa: E731
+    fd, vd, od = put(f), put(v), put(o)
+    hd = None if h is None else h.to(DEV).requires_grad_(True)
+    ld = None if lengths is None else lengths.to(DEV)
+    y, last = hn.gated_recurrence(fd, vd, out_gate=od, h0=hd, lengths=ld, direction=direction)
+    with torch.no_grad():
+        y2, last2 = hn.gated_recurrence(fd, vd, out_gate=od, h0=hd, lengths=ld, direction=direction)
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+    assert y.dtype == f.dtype and last.dtype == torch.float32
+    leaves = [t for t in (fd, vd, od, hd) if t is not None]
+    names = [n for n, t in zip(("df", "dv", "do", "dh0"), (fd, vd, od, hd)) if t is not None]
+    grads = torch.autograd.grad((y, last), leaves, (place(dy), dlast.to(DEV)))
+    for n, t in zip(["y", "last"] + names, (y, last) + grads):
+        _near(n, t, want[n], off[n])
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("direction", ["forward", "reverse", "both"])
+@pytest.mark.parametrize("T,B,C", [(1, 1, 2), (2, 3, 4), (7, 2, 130), (256, 1, 64), (257, 2, 36), (600, 1, 6), (1100, 3, 16)])
+def test_recurrence(T, B, C, direction, name):
+    _rec_check(_rec_case(T, B, C, DT[name]), direction, name)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("T,B,C,gate,h0", [(300, 2, 5, True, True), (33, 1, 1, False, False), (513, 2, 8, False, True), (20, 2, 12, True, False)])
+def test_recurrence_optional_inputs_and_odd_channels(T, B, C, gate, h0, name):
+    _rec_check(_rec_case(T, B, C, DT[name], gate, h0), "reverse" if C == 5 else "forward", name)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("direction", ["forward", "reverse", "both"])
+def test_recurrence_ragged(direction, name):
+    """Lengths of 0, 1, a tile's edge and past the end; what lies behind a length is never looked at."""
+    T, B, C = 600, 8, 8
+    lengths = torch.tensor([0, 1, 255, 256, 257, 599, 600, 9999], dtype=torch.int32)
+    case = list(_rec_case(T, B, C, DT[name], lengths=lengths))
+    for i in (0, 1, 2, 4):                                    # f, v, o, dy
+        for b, n in enumerate(lengths.tolist()):
+            case[i][n:, b] = float("nan") if i % 2 else float("inf")
+    poisoned = [t.clone() if isinstance(t, torch.Tensor) else t for t in case]
+    for i in (0, 1, 2, 4):
+        case[i] = torch.where(torch.isfinite(case[i]), case[i], torch.zeros((), dtype=DT[name]))
+    f, v, o, h, dy, dlast, _ = case
+    want, off = ref.recurrence(f, v, o, h, lengths, direction, dy, dlast, EPS[name])
+    leaves = [poisoned[i].to(DEV).requires_grad_(True) for i in (0, 1, 2, 3)]
+    y, last = hn.gated_recurrence(leaves[0], leaves[1], out_gate=leaves[2], h0=leaves[3], lengths=lengths.to(DEV), direction=direction)
+    grads = torch.autograd.grad((y, last), leaves, (poisoned[4].to(DEV), dlast.to(DEV)))
+    for n, t in zip(("y", "last", "df", "dv", "do", "dh0"), (y, last) + grads):
+        _near(n, t, want[n], off[n])
+    with torch.no_grad():                                     # 64-bit lengths are the same lengths
+        y2, _ = hn.gated_recurrence(leaves[0], leaves[1], out_gate=leaves[2], h0=leaves[3], lengths=lengths.long().to(DEV) + (1 << 40) * (lengths > 600).to(DEV),
+                                    direction=direction)
+    assert torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_recurrence_layouts(name):
+    """Parts of one projection's output, a batch-first tensor, odd offsets and strides, repeated rows: the same bits as packed inputs."""
+    T, B, C = 270, 3, 20
+    f, v, o, h, dy, dlast, _ = _rec_case(T, B, C, DT[name])
+    _rec_check((f, v, o, h, dy, dlast, None), "both", name, place=lambda t: t.to(DEV).transpose(0, 1).contiguous().transpose(0, 1))
+    wide = torch.cat([f, v, o], -1).to(DEV)
+    y, last = hn.gated_recurrence(f.to(DEV), v.to(DEV), out_gate=o.to(DEV))
+    parts = [wide[..., i * C:(i + 1) * C] for i in range(3)]
+    y2, last2 = hn.gated_recurrence(parts[0], parts[1], out_gate=parts[2])
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+    odd = torch.zeros(T, B, 3 * C + 5, dtype=DT[name], device=DEV)
+    odd[..., 1:1 + 3 * C] = wide                              # no vector access is aligned here
+    parts = [odd[..., 1 + i * C:1 + (i + 1) * C] for i in range(3)]
+    y3, last3 = hn.gated_recurrence(parts[0], parts[1], out_gate=parts[2])
+    want, off = ref.recurrence(f, v, o, None, None, "forward", eps=EPS[name])
+    _near("y", y3, want["y"], off["y"])
+    _near("last", last3, want["last"], off["last"])
+    across = [t.to(DEV).permute(2, 0, 1).contiguous().permute(1, 2, 0) for t in (f, v, o)]
+    y4, _ = hn.gated_recurrence(across[0], across[1], out_gate=across[2])
+    assert torch.equal(y, y4)
+    one = f[:1, :1].to(DEV).requires_grad_(True)              # a gate shared by all steps and sequences: its gradient is the sum
+    vd = v.to(DEV)
+    y5, last5 = hn.gated_recurrence(one.expand(T, B, C), vd)
+    full = f[:1, :1].expand(T, B, C)
+    want, off = ref.recurrence(full, v, None, None, None, "forward", dy, dlast, EPS[name])
+    got, = torch.autograd.grad((y5, last5), [one], (dy.to(DEV), dlast.to(DEV)))
+    _near("y", y5, want["y"], off["y"])
+    # each term is rounded to the type, and so are the partial sums of the broadcast's own adjoint (at most T * B of them)
+    terms = want["df"].abs() + off["df"]
+    half = ref.rounding(DT[name])
+    _near("shared df", got, want["df"].sum((0, 1), keepdim=True), (off["df"] + half * terms).sum((0, 1), keepdim=True) + 8 * half * terms.sum((0, 1), keepdim=True))
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_recurrence_only_one_gradient_path(name):
+    """Only y, or only h_last, is used."""
+    f, v, o, h, dy, dlast, _ = _rec_case(300, 2, 8, DT[name])
+    for use_y in (True, False):
+        want, off = ref.recurrence(f, v, o, h, None, "forward", dy if use_y else None, None if use_y else dlast, EPS[name])
+        leaves = [t.to(DEV).requires_grad_(True) for t in (f, v, o, h)]
+        y, last = hn.gated_recurrence(leaves[0], leaves[1], out_gate=leaves[2], h0=leaves[3])
+        grads = torch.autograd.grad(y if use_y else last, leaves, dy.to(DEV) if use_y else dlast.to(DEV))
+        for n, t in zip(("df", "dv", "do", "dh0"), grads):
+            _near(n, t, want[n], off[n])
+
+
+def test_recurrence_long_memory():
+    """a so near 1 that 1 - a is lost in a float32 a: the update still has its full precision."""
+    T, C = 2048, 4
+    f = torch.full((T, 1, C), 18.0)
+    v = torch.ones(T, 1, C)
+    _rec_check((f, v, None, torch.zeros(1, C), torch.ones(T, 1, C), torch.ones(1, C), None), "forward", "f32")
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_recurrence_saturated_gates(name):
+    """Gates at the type's largest and lowest values and at infinity keep or replace the state exactly."""
+    T, B, C = 5, 1, 4
+    big = torch.finfo(DT[name]).max
+    f = torch.tensor([big, -big, float("inf"), -float("inf"), big], dtype=DT[name]).view(T, 1, 1).expand(T, B, C).contiguous()
+    v = torch.arange(1, T + 1, dtype=DT[name]).view(T, 1, 1).expand(T, B, C).contiguous()
+    y, last = hn.gated_recurrence(f.to(DEV), v.to(DEV), h0=torch.full((B, C), 9.0, device=DEV))
+    assert y[:, 0, 0].tolist() == [9.0, 2.0, 2.0, 4.0, 4.0] and last[0, 0].item() == 4.0
+
+
+def test_recurrence_nothing_to_do():
+    for dtype in DT.values():
+        z = torch.zeros(0, 3, 4, dtype=dtype, device=DEV, requires_grad=True)
+        h = torch.randn(3, 4, device=DEV, requires_grad=True)
+        y, last = hn.gated_recurrence(z, z, h0=h)
+        assert y.shape == (0, 3, 4) and torch.equal(last, h)
+        gz, gh = torch.autograd.grad((y, last), [z, h], (torch.zeros_like(y), torch.ones_like(last)))
+        assert gz.shape == z.shape and torch.equal(gh, torch.ones_like(h))
+        assert torch.equal(hn.gated_recurrence(z, z)[1], torch.zeros(3, 4, device=DEV))
+        for shape in ((3, 0, 4), (3, 2, 0)):
+            e = torch.zeros(shape, dtype=dtype, device=DEV)
+            assert hn.gated_recurrence(e, e)[0].shape == shape
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("B,C", [(1, 1), (3, 130), (5, 64)])
+def test_recurrence_step(B, C, name):
+    """T single steps are the sequence."""
+    T = 9
+    f, v, o, h, _, _, _ = _rec_case(T, B, C, DT[name])
+    want, off = ref.recurrence(f, v, o, h, None, "forward", eps=EPS[name])
+    wide = torch.cat([f, v, o], -1).to(DEV)
+    state = h.to(DEV)
+    for t in range(T):
+        y = hn.gated_recurrence_step(wide[t, :, :C], wide[t, :, C:2 * C], state, out_gate=wide[t, :, 2 * C:])
+        _near("y", y, want["y"][t], off["y"][t])
+    _near("state", state, want["last"], off["last"])
+    before = state.clone()
+    y = hn.gated_recurrence_step(f[0].to(DEV), v[0].to(DEV), state)
+    assert torch.equal(y, state.to(DT[name])) and not torch.equal(state, before)
+
+
+def test_recurrence_far_offsets():
+    """Strides that carry an element's offset past 2**32."""
+    T, C, far = 3, 8, (1 << 31) + 8
+    store = torch.empty(2 * far + 64, dtype=torch.bfloat16, device=DEV)
+    f, v, o, _, dy, dlast, _ = _rec_case(T, 1, C, torch.bfloat16, h0=False)
+    views = []
+    for i, t in enumerate((f, v, o, dy)):
+        w = store[16 * i:].as_strided((T, 1, C), (far, C, 1))
+        w.copy_(t)
+        views.append(w)
+    want, off = ref.recurrence(f, v, o, None, None, "forward", dy, dlast, EPS["bf16"])
+    leaves = [w.detach().requires_grad_(True) for w in views[:3]]
+    y, last = hn.gated_recurrence(leaves[0], leaves[1], out_gate=leaves[2])
+    for n, t in zip(("y", "last", "df", "dv", "do"), (y, last) + torch.autograd.grad((y, last), leaves, (views[3], dlast.to(DEV)))):
+        _near(n, t, want[n], off[n])
+
+
+# ---- gated linear block ----
+def _lin_check(M, K, F, name, act, bias, place=lambda t: t.to(DEV), seed=0):
+    g = torch.Generator().manual_seed(seed + M + 3 * K + 5 * F)
+    dt = DT[name]
+    x, dy = _normal(g, M, K, dtype=dt), _normal(g, M, F, dtype=dt)
+    wg, wu = (_normal(g, F, K, dtype=dt, scale=max(K, 1) ** -0.5) for _ in range(2))
+    bg, bu = (_normal(g, F, dtype=dt) if bias & bit else None for bit in (1, 2))
+    want, off = ref.linear(x, wg, wu, bg, bu, act, dy)
+    put = lambda t: None if t is None else place(t).detach().requires_grad_(True)  # noqa: E731
+    args = [put(t) for t in (x, wg, wu)] + [None if t is None else t.to(DEV).requires_grad_(True) for t in (bg, bu)]
+    y = hn.gated_linear(*args, activation=act)
+    with torch.no_grad():
+        assert torch.equal(y, hn.gated_linear(*args, activation=act))
+    _near("y", y, want["y"], off["y"])
+    names = [n for n, t in zip(("dx", "dwg", "dwu", "dbg", "dbu"), args) if t is not None]
+    leaves = [t for t in args if t is not None]
+    grads = torch.autograd.grad(y, leaves, place(dy), retain_graph=True)
+    again = torch.autograd.grad(y, leaves, place(dy))
+    for n, t, t2 in zip(names, grads, again):
+        _near(n, t, want[n], off[n])
+        assert torch.equal(t, t2), n
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "relu"])
+@pytest.mark.parametrize("M,K,F", [(1, 8, 8), (5, 64, 33), (70, 40, 130)])
+def test_linear(M, K, F, act, name):
+    _lin_check(M, K, F, name, act, 3)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,F", [(1, 1, 1), (2, 1024, 520), (3, 7, 129), (16, 72, 64), (17, 128, 72), (63, 63, 65), (64, 64, 64), (128, 256, 128), (129, 200, 257),
+                                   (255, 31, 64), (257, 72, 264), (300, 520, 136), (513, 96, 48), (1000, 16, 24)])
+def test_linear_sizes(M, K, F, name):
+    _lin_check(M, K, F, name, "silu", 0)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("bias", [1, 2])
+def test_linear_one_bias(bias, name):
+    _lin_check(40, 24, 56, name, "gelu", bias)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_linear_layouts(name):
+    """Rows with a stride of their own, at an odd offset, and transposed weights."""
+    def padded(t):
+        return torch.cat([t.new_full((t.shape[0], 3), float("nan")), t, t.new_full((t.shape[0], 6), float("nan"))], 1).to(DEV)[:, 3:3 + t.shape[1]]
+
+    for M, K, F in ((37, 48, 80), (130, 64, 144), (4, 256, 96)):
+        _lin_check(M, K, F, name, "silu", 3, place=padded)
+        _lin_check(M, K, F, name, "silu", 3, place=lambda t: torch.cat([t, t.new_full((t.shape[0], 16), float("nan"))], 1).to(DEV)[:, :t.shape[1]])
+        _lin_check(M, K, F, name, "silu", 3, place=lambda t: t.t().contiguous().to(DEV).t())
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_linear_shapes_and_some_gradients(name):
+    g = torch.Generator().manual_seed(3)
+    x, wg, wu = _normal(g, 2, 3, 5, 24, dtype=DT[name]), _normal(g, 16, 24, dtype=DT[name]), _normal(g, 16, 24, dtype=DT[name])
+    dy = _normal(g, 2, 3, 5, 16, dtype=DT[name])
+    want, off = ref.linear(x.reshape(-1, 24), wg, wu, None, None, "silu", dy.reshape(-1, 16))
+    dev = [t.to(DEV) for t in (x, wg, wu)]
+    y = hn.gated_linear(*dev)
+    assert y.shape == (2, 3, 5, 16) and hn.gated_linear(dev[0][0, 0, 0], dev[1], dev[2]).shape == (16,)
+    _near("y", y.reshape(-1, 16), want["y"], off["y"])
+    for i, n in enumerate(("dx", "dwg", "dwu")):              # one gradient at a time
+        args = [t.clone().requires_grad_(i == j) for j, t in enumerate(dev)]
+        got, = torch.autograd.grad(hn.gated_linear(*args), [args[i]], dy.to(DEV))
+        _near(n, got.reshape(want[n].shape), want[n], off[n])
+    w = wg.to(DEV).requires_grad_(True)                       # one matrix as both weights, one row as all rows
+    row = x[0, 0, :1].to(DEV).requires_grad_(True)
+    y = hn.gated_linear(row.expand(30, 24), w, w)
+    got = torch.autograd.grad(y, [w, row], dy.reshape(30, 16).to(DEV))
+    want, off = ref.linear(x[0, 0, :1].expand(30, 24), wg, wg, None, None, "silu", dy.reshape(30, 16))
+    half = ref.rounding(DT[name])
+    terms = want["dwg"].abs() + want["dwu"].abs() + off["dwg"] + off["dwu"]
+    _near("shared dw", got[0], want["dwg"] + want["dwu"], off["dwg"] + off["dwu"] + half * terms)
+    terms = (want["dx"].abs() + off["dx"]).sum(0, keepdim=True)
+    _near("shared dx", got[1], want["dx"].sum(0, keepdim=True), off["dx"].sum(0, keepdim=True) + 8 * half * terms)
+
+
+def test_linear_nothing_to_do():
+    for dtype in DT.values():
+        for M, K, F in ((0, 8, 8), (3, 0, 8), (3, 8, 0)):
+            x, w, b = (torch.ones(s, dtype=dtype, device=DEV, requires_grad=True) for s in ((M, K), (F, K), (F,)))
+            y = hn.gated_linear(x, w, w, b, b, activation="relu")
+            assert y.shape == (M, F) and (K or bool((y == 1).all()))
+            dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.ones_like(y))
+            assert bool((dx == 0).all()) and bool((dw == 0).all()) if K == 0 or M == 0 or F == 0 else True
+            assert bool((db == (0 if M == 0 else 2 * M)).all())
+
+
+def test_linear_infinities_stay_in_their_row_and_column():
+    x = torch.ones(70, 64, device=DEV, dtype=torch.bfloat16)
+    w = torch.full((80, 64), 0.25, device=DEV, dtype=torch.bfloat16)
+    x[5, 3] = float("inf")
+    w2 = w.clone()
+    w2[7, 1] = float("nan")
+    y = hn.gated_linear(x, w, w2)
+    bad = ~torch.isfinite(y)
+    assert bool(bad[5].all()) and bool(bad[:, 7].all())
+    bad[5] = False
+    bad[:, 7] = False
+    assert not bool(bad.any())
+
+
+def test_linear_far_offsets():
+    K, far = 64, (1 << 31) + 64
+    store = torch.empty(2 * far + 64, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator().manual_seed(9)
+    x, wg, wu, dy = (_normal(g, *s, dtype=torch.bfloat16) for s in ((3, K), (72, K), (72, K), (3, 72)))
+    xv = store.as_strided((3, K), (far, 1))
+    xv.copy_(x)
+    leaves = [t.detach().requires_grad_(True) for t in (xv, wg.to(DEV), wu.to(DEV))]
+    want, off = ref.linear(x, wg, wu, None, None, "silu", dy)
+    y = hn.gated_linear(*leaves)
+    _near("y", y, want["y"], off["y"])
+    for n, t in zip(("dx", "dwg", "dwu"), torch.autograd.grad(y, leaves, dy.to(DEV))):
+        _near(n, t, want[n], off[n])
+
+
+# ---- dropout ----
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1,), (3,), (7, 5), (4, 64), (1023,), (256, 2, 130)])
+@pytest.mark.parametrize("p,residual,seed", [(0.5, False, 0), (0.1, True, 123), (0.9, True, 2 ** 64 - 1), (0.0, False, 5)])
+def test_dropout(shape, p, residual, seed, name):
+    g = torch.Generator().manual_seed(4)
+    x, r, dy = (_normal(g, *shape, dtype=DT[name]) for _ in range(3))
+    keep = ref.dropout_keep(x.numel(), p, seed).view(shape)
+    x[~keep] = float("nan")                                   # a dropped element is never looked at
+    clean = torch.where(keep, x, torch.zeros((), dtype=DT[name]))
+    want, off = ref.dropout(clean, p, seed, r if residual else None)
+    for s in [seed] + ([torch.tensor([seed], device=DEV)] if seed < 2 ** 63 else []):
+        xd, rd = x.to(DEV).requires_grad_(True), r.to(DEV).requires_grad_(True) if residual else None
+        y = hn.dropout(xd, p, s, residual=rd)
+        _near("y", y, want, off)
+        grads = torch.autograd.grad(y, [xd] + ([rd] if residual else []), dy.to(DEV))
+        _near("dx", grads[0], *ref.dropout(dy, p, seed))
+        if residual:
+            assert torch.equal(grads[1].cpu(), dy)
+
+
+def test_dropout_views():
+    """The mask goes by the position in the tensor as it is read, whatever lies between its elements."""
+    x = torch.randn(6, 9, 40, device=DEV)
+    assert torch.equal(hn.dropout(x.transpose(0, 2), 0.3, 11), hn.dropout(x.transpose(0, 2).contiguous(), 0.3, 11))
+    assert torch.equal(hn.dropout(x[1:, 1:, 1:], 0.3, 11), hn.dropout(x[1:, 1:, 1:].contiguous(), 0.3, 11))
+    flat = x.reshape(-1)
+    part = flat[1:1001]                                       # contiguous, at an odd offset
+    assert torch.equal(hn.dropout(part, 0.3, 11, residual=flat[3:1003]), hn.dropout(part.clone(), 0.3, 11, residual=flat[3:1003].clone()))
+
+
+def test_dropout_beyond_32_bits():
+    n = (1 << 32) + 1000
+    x = torch.ones(n, dtype=torch.bfloat16, device=DEV)
+    y = hn.dropout(x, 0.5, 77)
+    for at in (0, (1 << 31) - 500, (1 << 32) - 500, (1 << 32) + 400):
+        m = min(1000, n - at)
+        assert torch.equal(y[at:at + m].cpu(), ref.dropout_keep(m, 0.5, 77, at).to(torch.bfloat16) * 2)
+
+
+# ---- all of them ----
+def test_refusals():
+    x = torch.zeros(4, 2, 8, device=DEV)
+    b = x.bfloat16()
+    bad = [
+        (ValueError, lambda: hn.gated_recurrence(x.half(), x.half())), (ValueError, lambda: hn.gated_recurrence(x, b)),
+        (ValueError, lambda: hn.gated_recurrence(x, x[:3])), (ValueError, lambda: hn.gated_recurrence(x[0], x[0])),
+        (ValueError, lambda: hn.gated_recurrence(x, x, direction="sideways")), (ValueError, lambda: hn.gated_recurrence(x[..., :7], x[..., :7], direction="both")),
+        (ValueError, lambda: hn.gated_recurrence(x, x, out_gate=b)), (ValueError, lambda: hn.gated_recurrence(x, x, h0=x[0].bfloat16())),
+        (ValueError, lambda: hn.gated_recurrence(x, x, h0=x[0, :1])), (RuntimeError, lambda: hn.gated_recurrence(x, x.cpu())),
+        (RuntimeError, lambda: hn.gated_recurrence(x, x, h0=x[0].cpu())), (TypeError, lambda: hn.gated_recurrence(x, x, lengths=[1, 2])),
+        (TypeError, lambda: hn.gated_recurrence(x, x, lengths=torch.ones(2, device=DEV))), (RuntimeError, lambda: hn.gated_recurrence(x, x, lengths=torch.ones(2).int())),
+        (ValueError, lambda: hn.gated_recurrence(x, x, lengths=torch.ones(3, device=DEV).int())),
+        (ValueError, lambda: hn.gated_recurrence_step(x, x, x)), (ValueError, lambda: hn.gated_recurrence_step(x[0], x[0], b[0])),
+        (ValueError, lambda: hn.gated_recurrence_step(x[0], x[0], torch.zeros(8, 2, device=DEV).t())),
+        (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 7, device=DEV), torch.zeros(3, 7, device=DEV))),
+        (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(4, 8, device=DEV))),
+        (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(3, 8, device=DEV), activation="tanh")),
+        (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(3, 8, device=DEV), b_up=torch.zeros(4, device=DEV))),
+        (ValueError, lambda: hn.gated_linear(x.double(), torch.zeros(3, 8, device=DEV), torch.zeros(3, 8, device=DEV))),
+        (ValueError, lambda: hn.gated_linear(x, torch.zeros(8, device=DEV), torch.zeros(8, device=DEV))),
+        (RuntimeError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(3, 8))),
+        (ValueError, lambda: hn.dropout(x, 1.0, 1)), (ValueError, lambda: hn.dropout(x, -0.1, 1)), (ValueError, lambda: hn.dropout(x, float("nan"), 1)),
+        (ValueError, lambda: hn.dropout(x, 0.5, -1)), (ValueError, lambda: hn.dropout(x, 0.5, 1.5)), (ValueError, lambda: hn.dropout(x, 0.5, 1 << 64)),
+        (ValueError, lambda: hn.dropout(x, 0.5, torch.ones(2, dtype=torch.int64, device=DEV))), (ValueError, lambda: hn.dropout(x, 0.5, torch.ones(1, dtype=torch.int64))),
+        (ValueError, lambda: hn.dropout(x, 0.5, 1, residual=x[0])), (ValueError, lambda: hn.dropout(x, 0.5, 1, residual=b)),
+        (ValueError, lambda: hn.dropout(x.half(), 0.5, 1)),
+    ]
+    for i, (kind, call) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail("call %d of the list was taken" % i)
+
+
+def test_no_second_derivative_and_no_stale_inputs():
+    x = torch.randn(5, 2, 4, device=DEV, requires_grad=True)
+    y, _ = hn.gated_recurrence(x, x)
+    g, = torch.autograd.grad(y.sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [x])
+    seed = torch.tensor([3], device=DEV)
+    z = hn.dropout(x, 0.5, seed)
+    seed += 1                                                 # the backward pass would draw another mask
+    with pytest.raises(RuntimeError):
+        z.sum().backward()
+    state = torch.zeros(2, 4, device=DEV)
+    w = torch.randn(4, 4, device=DEV, requires_grad=True)
+    out = state @ w                                           # a graph that saved the state ...
+    hn.gated_recurrence_step(x[0].detach(), x[0].detach(), state)
+    with pytest.raises(RuntimeError):                         # ... notices that a step wrote it
+        out.sum().backward()
+
+
+class _Block:
+    """Projection -> gated recurrence (both directions) -> dropout + residual -> gated linear -> projection -> dropout + residual."""
+
+    def __init__(self, C, F, dtype, seed=6):
+        g = torch.Generator().manual_seed(seed)
+        n = lambda *s: _normal(g, *s, scale=s[-1] ** -0.5).to(dtype)  # noqa: E731
+        self.weights = {"p": n(3 * C, C), "wg": n(F, C), "wu": n(F, C), "down": n(C, F)}
+
+    def device(self, x, h0, lengths, w, seeds):
+        f, v, o = torch.nn.functional.linear(x, w["p"]).chunk(3, -1)
+        y, last = hn.gated_recurrence(f, v, out_gate=o, h0=h0, lengths=lengths, direction="both")
+        x = hn.dropout(y, 0.25, seeds[0], residual=x)
+        z = torch.nn.functional.linear(hn.gated_linear(x, w["wg"], w["wu"]), w["down"])
+        return hn.dropout(z, 0.1, seeds[1], residual=x), last
+
+    def oracle(self, x, h0, lengths, w, seeds):
+        """The same in plain differentiable float64."""
+        T, B, C = x.shape
+        f, v, o = torch.nn.functional.linear(x, w["p"]).chunk(3, -1)
+        live = (torch.arange(T)[:, None] < lengths[None])[..., None]
+        a, b = torch.sigmoid(f), torch.sigmoid(-f) * v
+        ys, ends = [], []
+        for half, order in ((slice(0, C // 2), range(T)), (slice(C // 2, C), range(T - 1, -1, -1))):
+            h, at = h0[:, half], {}
+            for t in order:
+                h = torch.where(live[t], a[t][:, half] * h + b[t][:, half], h)
+                at[t] = torch.where(live[t], torch.sigmoid(o[t][:, half]) * h, torch.zeros((), dtype=h.dtype))
+            ys.append(torch.stack([at[t] for t in range(T)]))
+            ends.append(h)
+        drop = lambda t, p, s: torch.where(ref.dropout_keep(t.numel(), p, s).view(t.shape), t / (1 - p), torch.zeros((), dtype=t.dtype))  # noqa: E731
+        x = x + drop(torch.cat(ys, -1), 0.25, seeds[0])
+        z = torch.nn.functional.silu(x @ w["wg"].t()) * (x @ w["wu"].t())
+        return x + drop(z @ w["down"].t(), 0.1, seeds[1]), torch.cat(ends, -1)
+
+
+def test_block_together():
+    """Forward and all gradients of two blocks in a row.  Norm-wise: a stage of float32 products over n <= 96 terms adds (n + 2) u = 6e-6 at
+    most, the 2 x 6 stages here have norms below 3 along a residual path, and the first errors pass through both blocks: 12 x 9 x 6e-6."""
+    T, B, C, F = 40, 3, 32, 96
+    block, g = _Block(C, F, torch.float32), torch.Generator().manual_seed(8)
+    x, dy, h0, dlast = _normal(g, T, B, C), _normal(g, T, B, C), _normal(g, B, C), _normal(g, B, C)
+    lengths = torch.tensor([40, 17, 0], dtype=torch.int32)
+
+    def both(fn, x, h0, lengths, w):
+        y, last = fn(x, h0, lengths, w, (11, 12))
+        return fn(y, last, lengths, w, (13, 14))
+
+    results = []
+    for fn, put in ((block.device, lambda t: t.to(DEV)), (block.oracle, lambda t: t.double())):
+        w = {k: put(t).requires_grad_(True) for k, t in block.weights.items()}
+        xs, hs = put(x).requires_grad_(True), put(h0).requires_grad_(True)
+        y, last = both(fn, xs, hs, lengths.to(xs.device), w)
+        grads = torch.autograd.grad((y, last), [xs, hs] + list(w.values()), (put(dy), put(dlast)))
+        results.append([t.detach().cpu().double() for t in (y, last) + grads])
+    for i, (a, b) in enumerate(zip(*results)):
+        assert float((a - b).norm() / b.norm()) < 12 * 9 * 6e-6, i
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_other_stream(name):
+    """Work enqueued on a side stream runs there, in order with what that stream does to the inputs before and after."""
+    f, v, o, h, _, _, _ = (None if t is None else t.to(DEV) for t in _rec_case(600, 2, 64, DT[name]))
+    w = torch.randn(96, 64, device=DEV).to(DT[name])
+    run = lambda f: (hn.gated_recurrence(f, v, out_gate=o, h0=h)[0], hn.gated_linear(f, w, w), hn.dropout(f, 0.5, 3, residual=v))  # noqa: E731
+    want = run(f * 0.5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            g = f.clone()
+            big = torch.randn(2048, 2048, device=DEV)
+            for _ in range(4):
+                big = big @ big * 1e-3                        # the stream is busy when the input is written
+            g.mul_(0.5)
+            got = run(g)
+            g.fill_(float("nan"))
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_captured_step(name):
+    """A block's forward and backward captured once and replayed with new inputs, states and seeds, eager work in between: every replay is
+    the eager result."""
+    T, B, C, F = 300, 2, 64, 96
+    block = _Block(C, F, DT[name])
+    w = {k: t.to(DEV).requires_grad_(True) for k, t in block.weights.items()}
+    x, h0 = torch.zeros(T, B, C, dtype=DT[name], device=DEV, requires_grad=True), torch.zeros(B, C, device=DEV, requires_grad=True)
+    lengths = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    seeds = torch.zeros(2, dtype=torch.int64, device=DEV)
+    dy, dlast = torch.zeros(T, B, C, dtype=DT[name], device=DEV), torch.zeros(B, C, device=DEV)
+
+    def step():
+        y, last = block.device(x, h0, lengths, w, (seeds[0:1].clone(), seeds[1:2].clone()))
+        return (y.detach(), last.detach()) + torch.autograd.grad((y, last), [x, h0] + list(w.values()), (dy, dlast))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    g = torch.Generator().manual_seed(10)
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(_normal(g, T, B, C))
+            h0.copy_(_normal(g, B, C))
+            dy.copy_(_normal(g, T, B, C))
+            dlast.copy_(_normal(g, B, C))
+            seeds.copy_(torch.tensor([100 + k, 200 + k]))
+            lengths.copy_(torch.tensor([T - 31 * k, 60 * k]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step()
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a, b), (k, i)
+
+
+def test_two_captured_graphs():
+    """Graphs of the same call replayed in turn on one stream do not share scratch memory."""
+    f = [torch.randn(2000, 1, 64, device=DEV) for _ in range(2)]
+    graphs, outs = [], []
+    for t in f:
+        hn.gated_recurrence(t, t)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(hn.gated_recurrence(t, t))
+        graphs.append(graph)
+    for k in range(3):
+        for t in f:
+            t.copy_(torch.randn(2000, 1, 64, device=DEV))
+        for graph in graphs:
+            graph.replay()
+        want = [hn.gated_recurrence(t, t) for t in f]
+        for a, b in zip(outs, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
