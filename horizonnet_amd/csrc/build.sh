@@ -12,7 +12,7 @@ mkdir -p $OBJDIR
 OBJS=""
 for f in $SRCS; do
   o=$OBJDIR/${f%.hip}.o
-  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ hn_common.h -nt "$o" ] || [ engine_internal.h -nt "$o" ] || [ multi_job.h -nt "$o" ] || [ conv_bf16_args.h -nt "$o" ] || [ conv_bf16_pp.h -nt "$o" ] || [ seq_common.h -nt "$o" ] || [ stat_commit.h -nt "$o" ] || [ stat_wave.h -nt "$o" ] || [ ../../include/horizonnet_hip.h -nt "$o" ]; then
+  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ hn_common.h -nt "$o" ] || [ engine_internal.h -nt "$o" ] || [ multi_job.h -nt "$o" ] || [ conv_bf16_args.h -nt "$o" ] || [ conv_bf16_pp.h -nt "$o" ] || [ seq_common.h -nt "$o" ] || [ gated_linear_tile.h -nt "$o" ] || [ stat_commit.h -nt "$o" ] || [ stat_wave.h -nt "$o" ] || [ ../../include/horizonnet_hip.h -nt "$o" ]; then
     case $f in
       conv_igemm_bf16_pp.hip|conv3x3_dwr_bf16.hip|conv3x3_dwr64_bf16.hip)
         # these kernels count their LDS-DMA queue by hand (s_waitcnt vmcnt(n), conv_bf16_pp.h): a scratch spill is a VMEM operation the

@@ -185,10 +185,11 @@ def _linear_forward(x, wg, wu, bg, bu, act):
     dev, (M, K), F = x.device, x.shape, wg.shape[0]
     lib, dt = _lib.load(), _DTYPES[x.dtype]
     y = torch.empty((M, F), dtype=x.dtype, device=dev)
-    n = lib.hn_gated_linear_workspace(M, K, F, dt, 0)
+    mats = (x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
+    n = lib.hn_gated_linear_workspace(*mats, M, K, F, dt, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with _on(dev):
-        _lib.check(lib.hn_gated_linear(x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), _addr(bg), _addr(bu), y.data_ptr(),
+        _lib.check(lib.hn_gated_linear(*mats, _addr(bg), _addr(bu), y.data_ptr(),
                                        _addr(ws), n, M, K, F, dt, act, _stream(dev)), "hn_gated_linear")
     return y
 
@@ -211,11 +212,11 @@ class _GatedLinear(torch.autograd.Function):
         new = lambda i, *shape: torch.empty(shape, dtype=x.dtype, device=dev) if need[i] else None  # noqa: E731
         dx, dwg, dwu = new(0, M, K), new(1, F, K), new(2, F, K)
         dbg, dbu = None if bg is None else new(3, F), None if bu is None else new(4, F)
-        n = lib.hn_gated_linear_workspace(M, K, F, dt, 1)
+        mats = (x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
+        n = lib.hn_gated_linear_workspace(*mats, M, K, F, dt, 1)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         with _on(dev):
-            _lib.check(lib.hn_gated_linear_bwd(x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), _addr(bg), _addr(bu),
-                                               dy.data_ptr(), dy.stride(0), _addr(dx), _addr(dwg), _addr(dwu), _addr(dbg), _addr(dbu), _addr(ws), n, M, K, F, dt,
+            _lib.check(lib.hn_gated_linear_bwd(*mats, _addr(bg), _addr(bu), dy.data_ptr(), dy.stride(0), _addr(dx), _addr(dwg), _addr(dwu), _addr(dbg), _addr(dbu), _addr(ws), n, M, K, F, dt,
                                                ctx.act, _stream(dev)), "hn_gated_linear_bwd")
         return dx, dwg, dwu, dbg, dbu, None
 
