@@ -93,7 +93,7 @@ SIGNATURES = {
     "hn_lstm_layer": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "hn_linear_head": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
     "hn_gated_recurrence_states": (_sz, [_i64, _i64, _i64]),
-    "hn_gated_recurrence_workspace": (_sz, [_i64, _i64, _i64]),
+    "hn_gated_recurrence_workspace": (_sz, [_i64, _i64, _i64, _i]),
     "hn_gated_recurrence": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
     "hn_gated_recurrence_bwd": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                      _i64, _i64, _i64, _i, _i, _vp]),

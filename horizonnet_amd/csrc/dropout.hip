@@ -8,7 +8,9 @@
 
 namespace {
 
-template <typename T, int VEC, bool RES>
+constexpr int VEC = 4;      // elements a thread takes at once
+
+template <typename T, bool RES>
 __global__ __launch_bounds__(256) void seq_dropout_kernel(const T* __restrict__ x, const T* __restrict__ r, T* __restrict__ y, long n, unsigned thr,
                                                           float scale, unsigned long long seed, const unsigned long long* seed_dev)
 {
@@ -16,7 +18,7 @@ __global__ __launch_bounds__(256) void seq_dropout_kernel(const T* __restrict__ 
     const long step = (long)gridDim.x * 256 * VEC;
     for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * VEC; i < n; i += step) {
         float a[VEC], b[VEC];
-        if (VEC == 1 || i + VEC <= n) {
+        if (i + VEC <= n) {
             seq_load<VEC>(x + i, a);
             if (RES) seq_load<VEC>(r + i, b);
 #pragma unroll
@@ -38,17 +40,17 @@ __global__ __launch_bounds__(256) void seq_dropout_kernel(const T* __restrict__ 
     }
 }
 
-template <typename T, int VEC>
+template <typename T>
 void dropout_launch(const void* x, const void* r, void* y, long n, unsigned thr, float scale, unsigned long long seed, const void* seed_dev, hipStream_t s)
 {
     long g = (n + 256L * VEC - 1) / (256L * VEC);
     if (g > 4096) g = 4096;
     const dim3 grid((unsigned)g);
     if (r)
-        hipLaunchKernelGGL((seq_dropout_kernel<T, VEC, true>), grid, dim3(256), 0, s, (const T*)x, (const T*)r, (T*)y, n, thr, scale, seed,
+        hipLaunchKernelGGL((seq_dropout_kernel<T, true>), grid, dim3(256), 0, s, (const T*)x, (const T*)r, (T*)y, n, thr, scale, seed,
                            (const unsigned long long*)seed_dev);
     else
-        hipLaunchKernelGGL((seq_dropout_kernel<T, VEC, false>), grid, dim3(256), 0, s, (const T*)x, (const T*)nullptr, (T*)y, n, thr, scale, seed,
+        hipLaunchKernelGGL((seq_dropout_kernel<T, false>), grid, dim3(256), 0, s, (const T*)x, (const T*)nullptr, (T*)y, n, thr, scale, seed,
                            (const unsigned long long*)seed_dev);
 }
 
@@ -62,16 +64,8 @@ extern "C" int hn_dropout(const void* x, const void* residual, void* y, int64_t 
     HN_REQUIRE(x && y, "hn_dropout: null pointer");
     const unsigned thr = (unsigned)((double)p * 4294967296.0);
     const float scale = 1.0f / (1.0f - p);
-    const size_t al = dtype == SEQ_F32 ? 16 : 8;
-    const bool v4 = (size_t)x % al == 0 && (size_t)residual % al == 0 && (size_t)y % al == 0;
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == SEQ_BF16) {
-        if (v4) dropout_launch<seq_bf16, 4>(x, residual, y, n, thr, scale, seed, seed_dev, s);
-        else dropout_launch<seq_bf16, 1>(x, residual, y, n, thr, scale, seed, seed_dev, s);
-    } else {
-        if (v4) dropout_launch<float, 4>(x, residual, y, n, thr, scale, seed, seed_dev, s);
-        else dropout_launch<float, 1>(x, residual, y, n, thr, scale, seed, seed_dev, s);
-    }
+    if (dtype == SEQ_BF16) dropout_launch<seq_bf16>(x, residual, y, n, thr, scale, seed, seed_dev, (hipStream_t)stream);
+    else dropout_launch<float>(x, residual, y, n, thr, scale, seed, seed_dev, (hipStream_t)stream);
     HN_LAUNCH_CHECK();
     return 0;
 }

@@ -18,48 +18,48 @@ __device__ __forceinline__ unsigned seq_pack2(float lo, float hi)
     return r;
 }
 
-template <int VEC>
-__device__ __forceinline__ void seq_load(const float* p, float (&x)[VEC])
+// VEC (1 or 4) neighbouring values as they lie in memory.  The vector types ask for no more than the element's own alignment: global memory is
+// read and written at any of them, so rows of an odd number of channels take the same wide accesses.
+typedef float seq_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short seq_u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T, int VEC>
+struct SeqRaw;
+template <>
+struct SeqRaw<float, 4> { typedef seq_f32x4u type; };
+template <>
+struct SeqRaw<float, 1> { typedef float type; };
+template <>
+struct SeqRaw<seq_bf16, 4> { typedef seq_u16x4u type; };
+template <>
+struct SeqRaw<seq_bf16, 1> { typedef seq_bf16 type; };
+
+__device__ __forceinline__ void seq_open(seq_f32x4u r, float (&x)[4]) { x[0] = r[0]; x[1] = r[1]; x[2] = r[2]; x[3] = r[3]; }
+__device__ __forceinline__ void seq_open(float r, float (&x)[1]) { x[0] = r; }
+__device__ __forceinline__ void seq_open(seq_u16x4u r, float (&x)[4])
 {
-    if constexpr (VEC == 4) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(p);
-        x[0] = t[0]; x[1] = t[1]; x[2] = t[2]; x[3] = t[3];
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) x[k] = p[k];
-    }
+    const uint2 t = __builtin_bit_cast(uint2, r);
+    x[0] = __builtin_bit_cast(float, t.x << 16); x[1] = __builtin_bit_cast(float, t.x & 0xffff0000u);
+    x[2] = __builtin_bit_cast(float, t.y << 16); x[3] = __builtin_bit_cast(float, t.y & 0xffff0000u);
 }
-template <int VEC>
-__device__ __forceinline__ void seq_load(const seq_bf16* p, float (&x)[VEC])
+__device__ __forceinline__ void seq_open(seq_bf16 r, float (&x)[1]) { x[0] = seq_from_bf16(r); }
+
+template <int VEC, typename T>
+__device__ __forceinline__ void seq_load(const T* p, float (&x)[VEC])
 {
-    if constexpr (VEC == 4) {
-        const uint2 t = *reinterpret_cast<const uint2*>(p);
-        x[0] = __builtin_bit_cast(float, t.x << 16); x[1] = __builtin_bit_cast(float, t.x & 0xffff0000u);
-        x[2] = __builtin_bit_cast(float, t.y << 16); x[3] = __builtin_bit_cast(float, t.y & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) x[k] = seq_from_bf16(p[k]);
-    }
+    seq_open(*reinterpret_cast<const typename SeqRaw<T, VEC>::type*>(p), x);
 }
-template <int VEC>
-__device__ __forceinline__ void seq_store(float* p, const float (&x)[VEC])
+__device__ __forceinline__ void seq_put(float* p, const float (&x)[4]) { *reinterpret_cast<seq_f32x4u*>(p) = seq_f32x4u{x[0], x[1], x[2], x[3]}; }
+__device__ __forceinline__ void seq_put(float* p, const float (&x)[1]) { *p = x[0]; }
+__device__ __forceinline__ void seq_put(seq_bf16* p, const float (&x)[4])
 {
-    if constexpr (VEC == 4) {
-        *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) p[k] = x[k];
-    }
+    const uint2 t = make_uint2(seq_pack2(x[0], x[1]), seq_pack2(x[2], x[3]));
+    *reinterpret_cast<seq_u16x4u*>(p) = __builtin_bit_cast(seq_u16x4u, t);
 }
-template <int VEC>
-__device__ __forceinline__ void seq_store(seq_bf16* p, const float (&x)[VEC])
+__device__ __forceinline__ void seq_put(seq_bf16* p, const float (&x)[1]) { *p = (seq_bf16)(seq_pack2(x[0], 0.f) & 0xffffu); }
+template <int VEC, typename T>
+__device__ __forceinline__ void seq_store(T* p, const float (&x)[VEC])
 {
-    if constexpr (VEC == 4) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(seq_pack2(x[0], x[1]), seq_pack2(x[2], x[3]));
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) p[k] = (seq_bf16)(seq_pack2(x[k], 0.f) & 0xffffu);
-    }
+    seq_put(p, x);
 }
 
 // s(x) and 1 - s(x) = s(-x) from ONE exponential of -|x|: neither is formed by a subtraction from 1, so the small one keeps its relative
@@ -73,6 +73,13 @@ __device__ __forceinline__ void seq_logistic(float x, float& s, float& rest)
     const float small = e * big;
     s = x >= 0.f ? big : small;
     rest = x >= 0.f ? small : big;
+}
+
+// s(x) alone: the exponential's overflow gives the right 0
+template <bool EXACT>
+__device__ __forceinline__ float seq_sigmoid(float x)
+{
+    return __builtin_amdgcn_rcpf(1.0f + (EXACT ? expf(-x) : __expf(-x)));
 }
 
 // The counter-based generator of every dropout here: 32 bits for element `index` of the stream base = seed * SEQ_DROPOUT_STRIDE (a 64-bit

@@ -31,18 +31,18 @@ class _Here:
 
 
 _HERE = _Here()
+# The public torch.cuda.current_device() / current_stream() cost 3 and 7 us in a call that is not in a tight loop, as much as a launch; these
+# are what they ask in turn.
+_device_now = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _on(device):
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _device_now() == device.index else torch.cuda.device(device)
 
 
 def _addr(t):
     return None if t is None else t.data_ptr()
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _check_main(who, name, t):
@@ -55,14 +55,15 @@ def _check_main(who, name, t):
 
 
 def _check_like(who, name, t, shape, dtype, device):
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == device:
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: %s must be a tensor" % (who, name))
     if t.device != device:
         raise RuntimeError("%s: %s is on %s, expected %s" % (who, name, t.device, device))
     if t.dtype != dtype:
         raise ValueError("%s: %s is %s, expected %s" % (who, name, t.dtype, dtype))
-    if t.shape != shape:
-        raise ValueError("%s: %s has shape %s, expected %s" % (who, name, tuple(t.shape), tuple(shape)))
+    raise ValueError("%s: %s has shape %s, expected %s" % (who, name, tuple(t.shape), tuple(shape)))
 
 
 def _rows(t):
@@ -80,12 +81,12 @@ def _recurrence_forward(f, v, o, h0, lengths, direction, keep):
     lib = _lib.load()
     y = torch.empty((T, B, C), dtype=f.dtype, device=dev)
     last = torch.empty((B, C), dtype=torch.float32, device=dev)
-    states = torch.empty(lib.hn_gated_recurrence_states(T, B, C), dtype=torch.float32, device=dev) if keep else None
-    n = lib.hn_gated_recurrence_workspace(T, B, C)
+    n = lib.hn_gated_recurrence_workspace(T, B, C, direction)
     ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    states = torch.empty(lib.hn_gated_recurrence_states(T, B, C), dtype=torch.float32, device=dev) if keep else None
     with _on(dev):
         _lib.check(lib.hn_gated_recurrence(*_tb(f), *_tb(v), *_tb(o), _addr(h0), _addr(lengths), y.data_ptr(), last.data_ptr(), _addr(states), _addr(ws), n,
-                                           T, B, C, _DTYPES[f.dtype], direction, _stream(dev)), "hn_gated_recurrence")
+                                           T, B, C, _DTYPES[f.dtype], direction, _raw_stream(dev.index)), "hn_gated_recurrence")
     return y, last, states
 
 
@@ -104,17 +105,17 @@ class _GatedRecurrence(torch.autograd.Function):
         f, v, o, lengths, states = ctx.saved_tensors
         dev, (T, B, C) = f.device, f.shape
         lib = _lib.load()
-        dy = torch.zeros((1, 1, 1), dtype=f.dtype, device=dev).expand(T, B, C).contiguous() if dy is None else _rows(dy)
+        dy = torch.zeros((T, B, C), dtype=f.dtype, device=dev) if dy is None else _rows(dy)
         dlast = None if dlast is None else dlast.contiguous()
-        df, dv = (torch.empty((T, B, C), dtype=f.dtype, device=dev) for _ in range(2))
-        d_o = None if o is None else torch.empty((T, B, C), dtype=f.dtype, device=dev)
+        grads = torch.empty((2 if o is None else 3, T, B, C), dtype=f.dtype, device=dev)      # one allocation: an allocation costs as much as a launch
+        df, dv, d_o = grads[0], grads[1], None if o is None else grads[2]
         dh0 = torch.empty((B, C), dtype=torch.float32, device=dev) if ctx.has_h0 else None
-        n = lib.hn_gated_recurrence_workspace(T, B, C)
+        n = lib.hn_gated_recurrence_workspace(T, B, C, ctx.direction)
         ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
         with _on(dev):
             _lib.check(lib.hn_gated_recurrence_bwd(*_tb(f), *_tb(v), *_tb(o), *_tb(dy), _addr(dlast), _addr(lengths), states.data_ptr(), df.data_ptr(),
                                                    dv.data_ptr(), _addr(d_o), _addr(dh0), _addr(ws), n, T, B, C, _DTYPES[f.dtype], ctx.direction,
-                                                   _stream(dev)), "hn_gated_recurrence_bwd")
+                                                   _raw_stream(dev.index)), "hn_gated_recurrence_bwd")
         return df, dv, d_o, dh0, None, None
 
 
@@ -155,7 +156,6 @@ def gated_recurrence(forget, value, out_gate=None, h0=None, lengths=None, direct
     return _recurrence_forward(f, v, o, h0, lengths, _DIRECTIONS[direction], False)[:2]
 
 
-@torch.no_grad()
 def gated_recurrence_step(forget, value, state, out_gate=None):
     """One step of ``gated_recurrence`` for a serving loop: forget, value, out_gate ``[B, C]``; state float32 ``[B, C]``, contiguous, is updated
     IN PLACE; returns y ``[B, C]``.  Not differentiable."""
@@ -175,7 +175,7 @@ def gated_recurrence_step(forget, value, state, out_gate=None):
     y = torch.empty((B, C), dtype=f.dtype, device=dev)
     with _on(dev):
         _lib.check(_lib.load().hn_gated_recurrence_step(f.data_ptr(), f.stride(0), v.data_ptr(), v.stride(0), _addr(o), 0 if o is None else o.stride(0),
-                                                        state.data_ptr(), y.data_ptr(), B, C, _DTYPES[f.dtype], _stream(dev)), "hn_gated_recurrence_step")
+                                                        state.data_ptr(), y.data_ptr(), B, C, _DTYPES[f.dtype], _raw_stream(dev.index)), "hn_gated_recurrence_step")
     torch.autograd.graph.increment_version(state)      # written behind torch's back: a graph that saved it must notice
     return y
 
@@ -190,7 +190,7 @@ def _linear_forward(x, wg, wu, bg, bu, act):
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     with _on(dev):
         _lib.check(lib.hn_gated_linear(*mats, _addr(bg), _addr(bu), y.data_ptr(),
-                                       _addr(ws), n, M, K, F, dt, act, _stream(dev)), "hn_gated_linear")
+                                       _addr(ws), n, M, K, F, dt, act, _raw_stream(dev.index)), "hn_gated_linear")
     return y
 
 
@@ -210,14 +210,18 @@ class _GatedLinear(torch.autograd.Function):
         dy = _rows(dy)
         need = ctx.needs_input_grad
         new = lambda i, *shape: torch.empty(shape, dtype=x.dtype, device=dev) if need[i] else None  # noqa: E731
-        dx, dwg, dwu = new(0, M, K), new(1, F, K), new(2, F, K)
+        dx = new(0, M, K)
+        if need[1] and need[2] and F * K % 8 == 0:
+            dwg, dwu = torch.empty((2, F, K), dtype=x.dtype, device=dev)      # one allocation for two results on 16 bytes
+        else:
+            dwg, dwu = new(1, F, K), new(2, F, K)
         dbg, dbu = None if bg is None else new(3, F), None if bu is None else new(4, F)
         mats = (x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0))
         n = lib.hn_gated_linear_workspace(*mats, M, K, F, dt, 1)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         with _on(dev):
             _lib.check(lib.hn_gated_linear_bwd(*mats, _addr(bg), _addr(bu), dy.data_ptr(), dy.stride(0), _addr(dx), _addr(dwg), _addr(dwu), _addr(dbg), _addr(dbu), _addr(ws), n, M, K, F, dt,
-                                               ctx.act, _stream(dev)), "hn_gated_linear_bwd")
+                                               ctx.act, _raw_stream(dev.index)), "hn_gated_linear_bwd")
         return dx, dwg, dwu, dbg, dbu, None
 
 
@@ -258,7 +262,7 @@ def _drop(x, residual, p, seed):
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     number, tensor = (0, seed) if isinstance(seed, torch.Tensor) else (seed, None)
     with _on(dev):
-        _lib.check(_lib.load().hn_dropout(x.data_ptr(), _addr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, number, _addr(tensor), _stream(dev)),
+        _lib.check(_lib.load().hn_dropout(x.data_ptr(), _addr(residual), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, number, _addr(tensor), _raw_stream(dev.index)),
                    "hn_dropout")
     return y
 

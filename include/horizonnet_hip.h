@@ -433,7 +433,7 @@ int hn_linear_head(const float* y, const float* w, const float* bias, float* bon
  * state passes (values outside 0 .. T count as the nearest).  y [T][B][C], h_last [B][C] = the state behind the last step taken.
  * states: hn_gated_recurrence_states() floats for hn_gated_recurrence_bwd, or null; workspace: hn_gated_recurrence_workspace() floats. */
 size_t hn_gated_recurrence_states(int64_t T, int64_t B, int64_t C);
-size_t hn_gated_recurrence_workspace(int64_t T, int64_t B, int64_t C);
+size_t hn_gated_recurrence_workspace(int64_t T, int64_t B, int64_t C, int direction);
 int hn_gated_recurrence(const void* f, int64_t f_t, int64_t f_b, const void* v, int64_t v_t, int64_t v_b, const void* o, int64_t o_t,
                         int64_t o_b, const float* h0, const int* lengths, void* y, float* h_last, float* states, float* workspace,
                         size_t workspace_floats, int64_t T, int64_t B, int64_t C, int dtype, int direction, void* stream);

@@ -90,8 +90,8 @@ def test_library_refusals():
     _fails(rec(C=1 << 31), "bad sizes")
     _fails(rec(y=None), "null pointer")
     _fails(rec(last=None), "null pointer")
-    _fails(rec(T=1000), "workspace too small")
-    _fails(rec(T=1000, n=1 << 20), "workspace too small")     # a size without an address
+    _fails(rec(T=5000), "workspace too small")
+    _fails(rec(T=5000, n=1 << 20), "workspace too small")     # a size without an address
     assert rec(B=0, y=None, last=None) == 0
     _fails(lib.hn_gated_recurrence_bwd(one, 16, 8, one, 16, 8, None, 0, 0, one, 16, 8, None, None, None, one, one, None, None, None, 0, 4, 2, 8, 0, 0, None),
            "null pointer")
