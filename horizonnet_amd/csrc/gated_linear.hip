@@ -10,47 +10,6 @@
 
 namespace {
 
-constexpr int ACT_SILU = 0, ACT_GELU = 1, ACT_SIGMOID = 2, ACT_RELU = 3;
-
-// value and slope of the activation
-template <bool EXACT>
-__device__ __forceinline__ void gl_act(float z, int act, float& a, float& slope)
-{
-    if (act == ACT_RELU) {
-        a = z > 0.f ? z : (z != z ? z : 0.f);
-        slope = z > 0.f ? 1.f : 0.f;
-    } else if (act == ACT_GELU) {
-        const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
-        a = z * cdf;
-        slope = fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), cdf);
-    } else {
-        float s, rest;
-        seq_logistic<EXACT>(z, s, rest);
-        if (act == ACT_SIGMOID) { a = s; slope = s * rest; }
-        else { a = z * s; slope = fmaf(z * s, rest, s); }
-    }
-}
-
-struct GlArgs {
-    GlOpd x, w;           // w: gate and up matrices
-    const void *bg, *bu, *dy;
-    long ldd;
-    void *y, *dgu;        // dgu: dg | du, rows of 2 Fp
-    float* slab;          // [row tiles][2F] column sums of dg | du, or null
-    long M, K, F, Fp;
-    int act, dy_vec, y_vec;
-};
-
-__device__ __forceinline__ float gl_ld(const float* p) { return *p; }
-__device__ __forceinline__ float gl_ld(const seq_bf16* p) { return seq_from_bf16(*p); }
-
-// neighbouring tiles (they share operands) on one XCD, which has an L2 of its own: workgroups go round the 8 XCDs
-__device__ __forceinline__ long gl_tile_of(long bid, long n)
-{
-    const long q = n >> 3, r = n & 7, xcd = bid & 7;
-    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
-}
-
 // both projections of TS rows x TS/2 hidden units, and y, or dg and du
 template <typename T, int TS, bool BWD>
 __global__ __launch_bounds__(256) void gl_gate_kernel(GlArgs p)
@@ -129,22 +88,6 @@ __global__ __launch_bounds__(256) void gl_gate_kernel(GlArgs p)
         }
     }
 }
-
-// a product of the backward pass: out[I][J] over `chunks` chunks of k, cut into `splits` runs of `run` chunks
-struct GlJob {
-    GlOpd a, b;
-    long I, J, K;         // K: k's of one source
-    int per, chunks, splits, run;
-    int a_kr;
-    int first;            // first workgroup
-    long tj, tiles;
-    void* out;
-    float* part;          // [splits][I][J] float32 where splits > 1
-};
-struct GlJobs {
-    GlJob j[3];
-    int n;
-};
 
 template <typename T, int TS>
 __global__ __launch_bounds__(256) void gl_product_kernel(GlJobs all)
@@ -233,7 +176,7 @@ int gl_check(int64_t M, int64_t K, int64_t F, int dtype, int act)
     HN_REQUIRE(M >= 0 && K >= 0 && F >= 0 && M < (1L << 31) && K < (1L << 24) && F < (1L << 24), "hn_gated_linear: bad sizes M=%ld K=%ld F=%ld", (long)M, (long)K,
                (long)F);
     HN_REQUIRE(dtype == SEQ_F32 || dtype == SEQ_BF16, "hn_gated_linear: dtype is 0 (float32) or 1 (bf16)");
-    HN_REQUIRE(act >= ACT_SILU && act <= ACT_RELU, "hn_gated_linear: activation is 0 (silu), 1 (gelu), 2 (sigmoid) or 3 (relu)");
+    HN_REQUIRE(act >= GL_SILU && act <= GL_RELU, "hn_gated_linear: activation is 0 (silu), 1 (gelu), 2 (sigmoid) or 3 (relu)");
     return 0;
 }
 
@@ -252,9 +195,10 @@ bool gl_aligned(const GlIn& in, const void* p, long ld) { return (size_t)p % 16 
 struct GlPlan {
     int ts_gate, ts_prod;
     size_t x, wg, wu, dgu, slab, part[3], bytes;      // offsets; 0-size parts share one
-    bool pack_x, pack_g, pack_u;
+    bool pack_x, pack_g, pack_u, pp_gate, pp_prod;
     int splits[3], run[3];
 };
+constexpr long GL_PP_TILES = 192;
 long gl_tiles(long I, long J, int ti, int tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); }
 
 GlPlan gl_plan(const GlIn& in, bool backward)
@@ -269,19 +213,24 @@ GlPlan gl_plan(const GlIn& in, bool backward)
     p.x = take(p.pack_x ? (size_t)M * gl_up8(K) * in.size : 0);
     p.wg = take(p.pack_g ? (size_t)F * gl_up8(K) * in.size : 0);
     p.wu = take(p.pack_u ? (size_t)F * gl_up8(K) * in.size : 0);
+    // the ping-pong tiles where they nearly fill the device; their loader's offsets are 32 bits over 256 rows
+    const long most = 1L << 22, ldx = p.pack_x ? gl_up8(K) : in.ldx, ldg = p.pack_g ? gl_up8(K) : in.ldg, ldu = p.pack_u ? gl_up8(K) : in.ldu;
+    const bool pp = in.size == 2 && ldx < most && ldg < most && ldu < most && F < most / 2;
+    p.pp_gate = pp && K >= 128 && gl_tiles(M, F, 256, 128) >= GL_PP_TILES;
     // the large tile where it still gives every compute unit a workgroup
     p.ts_gate = gl_tiles(M, F, 128, 64) >= 256 ? 128 : 64;
     if (backward) {
         p.dgu = take((size_t)M * 2 * gl_up8(F) * in.size);
         p.slab = take((size_t)((M + 63) / 64) * 2 * F * 4);
         const long I[3] = {M, F, F}, chunks[3] = {2 * ((F + bk - 1) / bk), (M + bk - 1) / bk, (M + bk - 1) / bk};
+        p.pp_prod = pp && ldg == ldu && M >= 128 && F >= 64 && gl_tiles(M, K, 256, 256) + 2 * gl_tiles(F, K, 256, 256) >= GL_PP_TILES;
         p.ts_prod = gl_tiles(M, K, 128, 128) + 2 * gl_tiles(F, K, 128, 128) >= 512 ? 128 : 64;
         for (int q = 0; q < 3; ++q) {
             // few tiles with a long k axis: runs of at least 4 chunks, as many as bring the product to 256 workgroups
             const long tiles = gl_tiles(I[q], K, p.ts_prod, p.ts_prod);
             long s = tiles > 0 ? 256 / tiles : 1;
             if (s > chunks[q] / 4) s = chunks[q] / 4;
-            if (s < 1) s = 1;
+            if (s < 1 || p.pp_prod) s = 1;
             p.run[q] = (int)((chunks[q] + s - 1) / s);
             if (p.run[q] < 1) p.run[q] = 1;
             p.splits[q] = (int)((chunks[q] + p.run[q] - 1) / p.run[q]);
@@ -377,6 +326,7 @@ int gl_forward(const GlIn& in, GlArgs p, char* ws, hipStream_t s)
 {
     const GlPlan pl = gl_plan(in, false);
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
+    if (pl.pp_gate) return hn_launch_gated_linear_pp_gate(p, false, s);
     return pl.ts_gate == 128 ? gl_gate<T, 128, false>(p, s) : gl_gate<T, 64, false>(p, s);
 }
 
@@ -385,12 +335,13 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
 {
     const GlPlan pl = gl_plan(in, true);
     const long bk = GlNum<T>::BK, Fp = p.Fp;
-    const int rows = pl.ts_gate;                                      // of a column-sum tile
+    const int rows = pl.pp_gate ? 128 : pl.ts_gate;                   // of a column-sum tile
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
     p.dgu = ws + pl.dgu;
     p.slab = dbg || dbu ? (float*)(ws + pl.slab) : nullptr;
     if (in.M > 0 && in.F > 0)
-        if (const int rc = pl.ts_gate == 128 ? gl_gate<T, 128, true>(p, s) : gl_gate<T, 64, true>(p, s)) return rc;
+        if (const int rc = pl.pp_gate ? hn_launch_gated_linear_pp_gate(p, true, s) : pl.ts_gate == 128 ? gl_gate<T, 128, true>(p, s) : gl_gate<T, 64, true>(p, s))
+            return rc;
     GlJobs jobs = {};
     void* outs[3] = {dx, dwg, dwu};
     for (int q = 0; q < 3; ++q) {
@@ -415,7 +366,7 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
         j.splits = pl.splits[q]; j.run = pl.run[q];
         j.part = (float*)(ws + pl.part[q]);
     }
-    if (const int rc = pl.ts_prod == 128 ? gl_products<T, 128>(jobs, s) : gl_products<T, 64>(jobs, s)) return rc;
+    if (const int rc = pl.pp_prod ? hn_launch_gated_linear_pp_products(jobs, s) : pl.ts_prod == 128 ? gl_products<T, 128>(jobs, s) : gl_products<T, 64>(jobs, s)) return rc;
     if ((dbg || dbu) && in.F > 0)
         hipLaunchKernelGGL((gl_bias_kernel<T>), dim3((unsigned)((2 * in.F + 255) / 256)), dim3(256), 0, s, p.slab, (in.M + rows - 1) / rows, in.F, (T*)dbg, (T*)dbu);
     HN_LAUNCH_CHECK();

@@ -9,22 +9,13 @@
 // v_mfma_f32_16x16x32_bf16 / v_mfma_f32_16x16x4_f32: lane l holds A row (B column) l % 16 at k group l / 16, and C column l % 16, rows
 // 4 (l / 16) .. + 3.  The order of k inside a chunk differs from memory order but is the same for both operands.
 #pragma once
-#include "seq_common.h"
+#include "gated_linear.h"
 
 namespace {
 
 typedef __bf16 gl_bf16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned int gl_u32x4 __attribute__((ext_vector_type(4)));
-typedef short gl_s16x4 __attribute__((ext_vector_type(4)));
 
 enum { GL_KC = 0, GL_KR = 1, GL_DUAL = 2 };      // GL_DUAL: KC rows, 16 of the first matrix and 16 of the second in turn
-
-// One operand.  Two sources: the two halves of a longer k axis, or the two matrices of GL_DUAL.
-struct GlOpd {
-    const void* p[2];
-    long ld[2];
-    long n;               // extent of the operand's own index
-};
 
 template <typename T>
 struct GlNum {
@@ -186,54 +177,6 @@ __device__ __forceinline__ void gl_dump(float* t, const f32x4 (&acc)[TS / 32][TS
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[((wi * N + i) * 16 + 4 * (lane >> 4) + r) * (TS + 4) + (wj * N + j) * 16 + (lane & 15)] = acc[i][j][r];
     __syncthreads();
-}
-
-// 8 neighbouring values of a row: one or two 16-byte accesses where `vec` says that the row allows it, else one by one up to `n`
-__device__ __forceinline__ void gl_store8(float* p, const float (&x)[8], bool vec, long n)
-{
-    if (vec && n >= 8) {
-        *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < n) p[e] = x[e];
-    }
-}
-__device__ __forceinline__ void gl_store8(seq_bf16* p, const float (&x)[8], bool vec, long n)
-{
-    if (vec && n >= 8) {
-        *reinterpret_cast<gl_u32x4*>(p) = gl_u32x4{seq_pack2(x[0], x[1]), seq_pack2(x[2], x[3]), seq_pack2(x[4], x[5]), seq_pack2(x[6], x[7])};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < n) p[e] = (seq_bf16)(seq_pack2(x[e], 0.f) & 0xffffu);
-    }
-}
-__device__ __forceinline__ void gl_load8(const float* p, float (&x)[8], bool vec, long n)
-{
-    if (vec && n >= 8) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = e < n ? p[e] : 0.f;
-    }
-}
-__device__ __forceinline__ void gl_load8(const seq_bf16* p, float (&x)[8], bool vec, long n)
-{
-    if (vec && n >= 8) {
-        const gl_u32x4 t = *reinterpret_cast<const gl_u32x4*>(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[2 * e] = __builtin_bit_cast(float, t[e] << 16);
-            x[2 * e + 1] = __builtin_bit_cast(float, t[e] & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = e < n ? seq_from_bf16(p[e]) : 0.f;
-    }
 }
 
 }  // namespace

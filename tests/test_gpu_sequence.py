@@ -249,6 +249,27 @@ def test_linear_sizes(M, K, F, name):
     _lin_check(M, K, F, name, "silu", 0)
 
 
+@pytest.mark.parametrize("M,K,F,bias,act", [(2048, 128, 4096, 0, "silu"), (4100, 200, 1544, 3, "gelu"), (3000, 1032, 2050, 3, "sigmoid"), (12345, 130, 520, 1, "relu"),
+                                            (600, 1024, 8200, 2, "silu"), (9000, 1096, 1000, 0, "silu")])
+def test_linear_large(M, K, F, bias, act):
+    """Sizes that take the large tiles, whole and ragged ones: checked against float64 on the device, at every element."""
+    g = torch.Generator(device=DEV).manual_seed(M)
+    n = lambda *s, scale=1.0: (torch.randn(*s, generator=g, device=DEV) * scale).bfloat16()  # noqa: E731
+    x, dy, wg, wu = n(M, K), n(M, F), n(F, K, scale=K ** -0.5), n(F, K, scale=K ** -0.5)
+    bg, bu = (n(F) if bias & bit else None for bit in (1, 2))
+    want, off = ref.linear(x, wg, wu, bg, bu, act, dy)        # (the oracle works where its inputs are)
+    args = [t if t is None else t.requires_grad_(True) for t in (x, wg, wu, bg, bu)]
+    y = hn.gated_linear(*args, activation=act)
+    leaves = [t for t in args if t is not None]
+    names = [k for k, t in zip(("dx", "dwg", "dwu", "dbg", "dbu"), args) if t is not None]
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    second = torch.autograd.grad(y, leaves, dy)
+    for k, t in zip(["y"] + names, (y,) + first):
+        _near(k, t, want[k].cpu(), off[k].cpu())
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("bias", [1, 2])
 def test_linear_one_bias(bias, name):
