@@ -9,17 +9,15 @@ OBJDIR=${HN_BUILD_OBJ:-../../build/obj}
 NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
 SRCS="engine.hip engine_bf16.hip train.hip conv_igemm_f32.hip conv_wgrad_f32.hip conv_wgrad_bf16.hip bn_fold.hip conv_igemm_bf16.hip conv_igemm_bf16_pp.hip conv3x3_dwr_bf16.hip conv3x3_dwr64_bf16.hip stem_pool_bf16.hip stem_pool_f32.hip elementwise.hip train_ops.hip lstm.hip lstm_wide_f32.hip lstm_bf16.hip panostretch.hip augment.hip labels.hip peaks.hip multi_job.hip layout_fit.hip probe.hip gated_recurrence.hip gated_linear.hip gated_linear_pp.hip dropout.hip"
 mkdir -p $OBJDIR
-OBJS=""
-for f in $SRCS; do
-  o=$OBJDIR/${f%.hip}.o
-  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ hn_common.h -nt "$o" ] || [ engine_internal.h -nt "$o" ] || [ multi_job.h -nt "$o" ] || [ conv_bf16_args.h -nt "$o" ] || [ conv_bf16_pp.h -nt "$o" ] || [ seq_common.h -nt "$o" ] || [ gated_linear.h -nt "$o" ] || [ gated_linear_tile.h -nt "$o" ] || [ stat_commit.h -nt "$o" ] || [ stat_wave.h -nt "$o" ] || [ ../../include/horizonnet_hip.h -nt "$o" ]; then
-    case $f in
-      conv_igemm_bf16_pp.hip|conv3x3_dwr_bf16.hip|conv3x3_dwr64_bf16.hip|gated_linear_pp.hip)
-        # these kernels count their LDS-DMA queue by hand (s_waitcnt vmcnt(n), conv_bf16_pp.h): a scratch spill is a VMEM operation the
-        # count does not know about, so a build whose hand-counted kernels spill is refused, not shipped
-        /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-pass-failed $NOPK ${HN_BUILD_FLAGS:-} -Rpass-analysis=kernel-resource-usage -c "$f" -o "$o" 2> "$o.usage" || { cat "$o.usage"; exit 1; }
-        grep -v 'kernel-resource-usage' "$o.usage" >&2 || true
-        python3 - "$o.usage" <<'PY' || { rm -f "$o"; exit 1; }
+compile() {      # source, object
+  local f=$1 o=$2
+  case $f in
+    conv_igemm_bf16_pp.hip|conv3x3_dwr_bf16.hip|conv3x3_dwr64_bf16.hip|gated_linear_pp.hip)
+      # these kernels count their LDS-DMA queue by hand (s_waitcnt vmcnt(n), conv_bf16_pp.h): a scratch spill is a VMEM operation the
+      # count does not know about, so a build whose hand-counted kernels spill is refused, not shipped
+      /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-pass-failed $NOPK ${HN_BUILD_FLAGS:-} -Rpass-analysis=kernel-resource-usage -c "$f" -o "$o" 2> "$o.usage" || { cat "$o.usage"; exit 1; }
+      grep -v 'kernel-resource-usage' "$o.usage" >&2 || true
+      python3 - "$o.usage" <<'PY' || { rm -f "$o"; exit 1; }
 import re, sys
 name, bad = None, []
 for line in open(sys.argv[1]):
@@ -31,14 +29,24 @@ for line in open(sys.argv[1]):
 for n, b in bad: print("build.sh: %s spills %d bytes/lane of scratch (hand-counted vmcnt kernels must not)" % (n, b))
 sys.exit(1 if bad else 0)
 PY
-        ;;
-      *)
-        /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-pass-failed $NOPK ${HN_BUILD_FLAGS:-} -c "$f" -o "$o"
-        ;;
-    esac
+      ;;
+    *)
+      /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-pass-failed $NOPK ${HN_BUILD_FLAGS:-} -c "$f" -o "$o"
+      ;;
+  esac
+}
+PIDS=""
+OBJS=""
+for f in $SRCS; do
+  o=$OBJDIR/${f%.hip}.o
+  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ hn_common.h -nt "$o" ] || [ engine_internal.h -nt "$o" ] || [ multi_job.h -nt "$o" ] || [ conv_bf16_args.h -nt "$o" ] || [ conv_bf16_pp.h -nt "$o" ] || [ seq_common.h -nt "$o" ] || [ gated_linear.h -nt "$o" ] || [ gated_linear_tile.h -nt "$o" ] || [ stat_commit.h -nt "$o" ] || [ stat_wave.h -nt "$o" ] || [ ../../include/horizonnet_hip.h -nt "$o" ]; then
+    compile "$f" "$o" &
+    PIDS="$PIDS $!"
+    if [ $(jobs -rp | wc -l) -ge ${HN_BUILD_JOBS:-8} ]; then wait -n || exit 1; fi
   fi
   OBJS="$OBJS $o"
 done
+for q in $PIDS; do wait $q || exit 1; done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT $OBJS
 echo "built $(readlink -f $OUT)"
 # an unresolved kernel stub only shows up at dlopen time: fail the build, not the first GPU call

@@ -44,7 +44,8 @@ int hn_launch_gated_linear_pp_products(GlJobs& jobs, hipStream_t s);
 
 namespace {
 
-// value and slope of the activation
+// Value and slope of the activation.  bf16 (not EXACT): the sigmoid from one exponential and one reciprocal, 1 - s by subtraction: what that
+// loses is far below the step of a bf16 result, which s and 1 - s enter beside terms of their own size.
 template <bool EXACT>
 __device__ __forceinline__ void gl_act(float z, int act, float& a, float& slope)
 {
@@ -57,9 +58,14 @@ __device__ __forceinline__ void gl_act(float z, int act, float& a, float& slope)
         slope = fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), cdf);
     } else {
         float s, rest;
-        seq_logistic<EXACT>(z, s, rest);
+        if constexpr (EXACT) {
+            seq_logistic<true>(z, s, rest);
+        } else {
+            s = seq_sigmoid<false>(z);
+            rest = 1.f - s;
+        }
         if (act == GL_SIGMOID) { a = s; slope = s * rest; }
-        else { a = z * s; slope = fmaf(z * s, rest, s); }
+        else { a = z * s; slope = fmaf(a, rest, s); }
     }
 }
 

@@ -62,8 +62,8 @@ __global__ __launch_bounds__(256) void gl_gate_kernel(GlArgs p)
                 for (int e = 0; e < 8; ++e) {
                     float a, slope;
                     gl_act<sizeof(T) == 4>(g[e], p.act, a, slope);
-                    g[e] = e < left ? d[e] * u[e] * slope : 0.f;      // (the columns up to Fp are read by the products: 0)
-                    u[e] = e < left ? d[e] * a : 0.f;
+                    g[e] = d[e] * u[e] * slope;                       // (0 in the columns up to Fp, which the products read: d is)
+                    u[e] = d[e] * a;
                     sg[e] += g[e];
                     su[e] += u[e];
                 }

@@ -143,13 +143,11 @@ __device__ __forceinline__ void gp_run(W& w, char* smem)
         }
     };
     f32x16 acc[4][2];
-    auto clear = [&]() {
+    auto clear = [&](float c0, float c1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+            for (int r = 0; r < 16; ++r) { acc[i][0][r] = c0; acc[i][1][r] = c1; }
     };
     auto mm = [&](int j) {
 #pragma unroll
@@ -158,7 +156,9 @@ __device__ __forceinline__ void gp_run(W& w, char* smem)
             for (int i = 0; i < 4; ++i)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fa[i][sh]), __builtin_bit_cast(bf16x8, fb[sh]), acc[i][j], 0, 0, 0);
     };
-    clear();
+    float c0 = 0.f, c1 = 0.f;             // what the sums of the lane's two columns start from: the biases
+    w.start(t, c0, c1);
+    clear(c0, c1);
 
     // chunk 0 whole, the A regions of chunk 1 (its B regions follow in phases 1 and 2 of chunk 0)
     issue_a(0, 0); issue_a(0, 1); issue_b(0, 0); issue_b(0, 1);
@@ -205,9 +205,10 @@ __device__ __forceinline__ void gp_run(W& w, char* smem)
             ckc = 0;
             if (g == 0) pp_bar_raw();         // the groups meet for the epilogue ...
             w.finish(t, acc, reinterpret_cast<float*>(smem + GP_SLAB + wave * 4096));
-            clear();
             vb += (int)gridDim.x;
             if (!w.tile(vb, t)) break;
+            w.start(t, c0, c1);
+            clear(c0, c1);
             if (g == 1) pp_bar_raw();         // ... and part again behind it
         }
     }
@@ -273,7 +274,7 @@ __device__ __forceinline__ void gp_slab_get(const float* slab, int row, int blk,
 }
 
 // ---- both projections ----
-template <bool BWD>
+template <bool BWD, int ACT>
 struct GpGate {
     const GlArgs& p;
     int nt, total, chunks;
@@ -303,70 +304,119 @@ struct GpGate {
         gp_aim_kc(c, p.F - t.j0, p.w.ld, p.K, chunks, [](int, int r) { return r; });
         return true;
     }
-    // a lane takes 8 hidden units of one of 16 rows: g from the left half of the slab's row, u from the right
+    __device__ __forceinline__ void start(const GpTile& t, float& c0, float& c1) const
+    {
+        const long f = t.j0 + 32 * (threadIdx.x >> 6 & 3) + (threadIdx.x & 31);
+        if (p.bg) c0 = f < p.F ? gl_ld((const seq_bf16*)p.bg + f) : 0.f;
+        if (p.bu) c1 = f < p.F ? gl_ld((const seq_bf16*)p.bu + f) : 0.f;
+    }
     __device__ __forceinline__ void finish(const GpTile& t, f32x16 (&acc)[4][2], float* slab) const
     {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gg = wave >> 2, wn = wave & 3;
-        const int row = lane >> 2, cq = lane & 3;
-        const long f = t.j0 + 32 * wn + 8 * cq, left = p.F - f, m0 = t.i0 + 128 * gg;
-        float bg[8], bu[8], sg[8], su[8];
+        const long m0 = t.i0 + 128 * gg;
+        const int row = lane >> 2, cq = lane & 3;             // of a store: 16 rows, 8 hidden units a lane
+        const long f = t.j0 + 32 * wn + 8 * cq, left = p.F - f;
+        if constexpr (!BWD) {
+            // the activation where the accumulators lie (a lane: one hidden unit, 64 rows), rounded, then turned in LDS 64 rows at a time: 64-byte
+            // rows, 16-byte units exchanged by row
+            seq_bf16* sh = reinterpret_cast<seq_bf16*>(slab);
+            const int fr = lane & 31, half = lane >> 5;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { bg[e] = bu[e] = sg[e] = su[e] = 0.f; }
-        if (p.bg) gl_load8((const seq_bf16*)p.bg + f, bg, false, left);
-        if (p.bu) gl_load8((const seq_bf16*)p.bu + f, bu, false, left);
-        float d[8];
+            for (int ih = 0; ih < 2; ++ih) {
 #pragma unroll
-        for (int rd = 0; rd < 8; ++rd) {
-            const long m = m0 + 16 * rd + row;
-            const bool on = m < p.M && left > 0;
-            if (BWD && on) gl_load8((const seq_bf16*)p.dy + m * p.ldd + f, d, p.dy_vec, left);
-            gp_slab_put(slab, acc, rd >> 1, rd & 1);
-            float gv[8], uv[8];
-            gp_slab_get(slab, row, 2 * cq, gv);
-            gp_slab_get(slab, row, 8 + 2 * cq, uv);
-            if (on) {
+                for (int i2 = 0; i2 < 2; ++i2)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float a, slope;
-                    const float u = uv[e] + bu[e];
-                    gl_act<false>(gv[e] + bg[e], p.act, a, slope);
-                    if (BWD) {
-                        gv[e] = e < left ? d[e] * u * slope : 0.f;
-                        uv[e] = e < left ? d[e] * a : 0.f;
-                        sg[e] += gv[e];
-                        su[e] += uv[e];
-                    } else {
-                        gv[e] = a * u;
+                    for (int r = 0; r < 16; r += 2) {
+                        const int i = 2 * ih + i2, lr = 32 * i2 + (r & 3) + 8 * (r >> 2) + 4 * half;      // rows lr, lr + 1
+                        float a0, a1, slope;
+                        gl_act<false>(acc[i][0][r], ACT, a0, slope);
+                        gl_act<false>(acc[i][0][r + 1], ACT, a1, slope);
+                        const unsigned v = seq_pack2(a0 * acc[i][1][r], a1 * acc[i][1][r + 1]);
+                        const int unit = ((fr >> 3) ^ (lr >> 2 & 3)) * 8 + (fr & 7);
+                        sh[lr * 32 + unit] = (seq_bf16)v;
+                        sh[(lr + 1) * 32 + unit] = (seq_bf16)(v >> 16);
+                    }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int lr = 16 * q + row;
+                    const long m = m0 + 64 * ih + lr;
+                    const gl_u32x4 v = *reinterpret_cast<const gl_u32x4*>(sh + lr * 32 + (cq ^ (lr >> 2 & 3)) * 8);
+                    if (m < p.M && left > 0) {
+                        if (p.y_vec && left >= 8) {
+                            *reinterpret_cast<gl_u32x4*>((seq_bf16*)p.y + m * p.F + f) = v;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const unsigned x = v[e >> 1];
+                                if (e < left) ((seq_bf16*)p.y)[m * p.F + f + e] = (seq_bf16)(e & 1 ? x >> 16 : x);
+                            }
+                        }
                     }
                 }
-                if (BWD) {
+            }
+        } else {
+            // 16 rows at a time through the slab: g in the left half of its rows, u in the right; the rows' dy two rounds ahead
+            float sg[8], su[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
+            const bool fast = p.dy_vec && t.i0 + 256 <= p.M && t.j0 + 128 <= p.F;      // (the whole tile exists)
+            gl_u32x4 ring[2];
+            const seq_bf16* pd = (const seq_bf16*)p.dy + (m0 + row) * p.ldd + f;
+            if (fast) {
+                ring[0] = *reinterpret_cast<const gl_u32x4*>(pd);
+                ring[1] = *reinterpret_cast<const gl_u32x4*>(pd + 16 * p.ldd);
+            }
+#pragma unroll
+            for (int rd = 0; rd < 8; ++rd) {
+                const long m = m0 + 16 * rd + row;
+                const bool on = m < p.M && left > 0;
+                float d[8], gv[8], uv[8];
+                gp_slab_put(slab, acc, rd >> 1, rd & 1);
+                gp_slab_get(slab, row, 2 * cq, gv);
+                gp_slab_get(slab, row, 8 + 2 * cq, uv);
+                if (fast) {
+                    gl_open8(ring[rd & 1], d);
+                    if (rd + 2 < 8) ring[rd & 1] = *reinterpret_cast<const gl_u32x4*>(pd + 16L * (rd + 2) * p.ldd);
+                } else if (on) {
+                    gl_load8((const seq_bf16*)p.dy + m * p.ldd + f, d, p.dy_vec, left);
+                }
+                if (on) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float a, slope;
+                        gl_act<false>(gv[e], ACT, a, slope);
+                        gv[e] = d[e] * uv[e] * slope;         // (0 in the columns up to Fp, which the products read: d is)
+                        uv[e] = d[e] * a;
+                    }
+                    if (p.slab) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) { sg[e] += gv[e]; su[e] += uv[e]; }
+                    }
                     gl_store8((seq_bf16*)p.dgu + m * 2 * p.Fp + f, gv, true, 8);
                     gl_store8((seq_bf16*)p.dgu + m * 2 * p.Fp + p.Fp + f, uv, true, 8);
-                } else {
-                    gl_store8((seq_bf16*)p.y + m * p.F + f, gv, p.y_vec, left);
                 }
             }
-        }
-        if (BWD && p.slab && m0 < p.M) {              // the 16 row lanes joined, one slab row per 128 rows
+            if (p.slab && m0 < p.M) {                         // the 16 row lanes joined, one slab row per 128 rows
 #pragma unroll
-            for (int st = 4; st < 64; st *= 2)
+                for (int st = 4; st < 64; st *= 2)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { sg[e] += __shfl_xor(sg[e], st, 64); su[e] += __shfl_xor(su[e], st, 64); }
-            if (row == 0 && left > 0) {
-                float* to = p.slab + m0 / 128 * 2 * p.F + f;
+                    for (int e = 0; e < 8; ++e) { sg[e] += __shfl_xor(sg[e], st, 64); su[e] += __shfl_xor(su[e], st, 64); }
+                if (row == 0 && left > 0) {
+                    float* to = p.slab + m0 / 128 * 2 * p.F + f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < left) { to[e] = sg[e]; to[p.F + e] = su[e]; }
+                    for (int e = 0; e < 8; ++e)
+                        if (e < left) { to[e] = sg[e]; to[p.F + e] = su[e]; }
+                }
             }
         }
     }
 };
 
-template <bool BWD>
+template <bool BWD, int ACT>
 __global__ __launch_bounds__(512) void gl_gate_pp_kernel(GlArgs p, int nt, int total)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    GpGate<BWD> w{p, nt, total, (int)((p.K + 63) >> 6)};
+    GpGate<BWD, ACT> w{p, nt, total, (int)((p.K + 63) >> 6)};
     gp_run<false, false>(w, smem);
 }
 
@@ -404,6 +454,7 @@ struct GpProduct {
         gp_aim_kr(c, p.b.n - t.j0, p.b.ld[0], p.K, p.chunks, [](int reg, int x) { return 64 * (x >> 5) + 32 * reg + (x & 31); });
         return true;
     }
+    __device__ __forceinline__ void start(const GpTile&, float&, float&) const {}
     __device__ __forceinline__ void finish(const GpTile& t, f32x16 (&acc)[4][2], float* slab) const
     {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gg = wave >> 2, wn = wave & 3;
@@ -454,16 +505,16 @@ int gp_ready(Kernel kern, bool (&told)[64], int& cus)
     return 0;
 }
 
-template <bool BWD>
+template <bool BWD, int ACT>
 int gp_gate(const GlArgs& p, hipStream_t s)
 {
     static bool told[64] = {};
     int cus = 256;
-    if (const int rc = gp_ready(gl_gate_pp_kernel<BWD>, told, cus)) return rc;
+    if (const int rc = gp_ready(gl_gate_pp_kernel<BWD, ACT>, told, cus)) return rc;
     const int nt = hn_cdiv(p.F, 128);
     const long total = (long)hn_cdiv(p.M, 256) * nt;
     HN_REQUIRE(total > 0 && total <= 0x3fffffffL, "hn_gated_linear: too many tiles");
-    hipLaunchKernelGGL((gl_gate_pp_kernel<BWD>), dim3((unsigned)(total < cus ? total : cus)), dim3(512), GP_LDS, s, p, nt, (int)total);
+    hipLaunchKernelGGL((gl_gate_pp_kernel<BWD, ACT>), dim3((unsigned)(total < cus ? total : cus)), dim3(512), GP_LDS, s, p, nt, (int)total);
     HN_LAUNCH_CHECK();
     return 0;
 }
@@ -472,7 +523,12 @@ int gp_gate(const GlArgs& p, hipStream_t s)
 
 int hn_launch_gated_linear_pp_gate(const GlArgs& p, bool backward, hipStream_t s)
 {
-    return backward ? gp_gate<true>(p, s) : gp_gate<false>(p, s);
+    switch (p.act) {
+    case GL_SILU: return backward ? gp_gate<true, GL_SILU>(p, s) : gp_gate<false, GL_SILU>(p, s);
+    case GL_GELU: return backward ? gp_gate<true, GL_GELU>(p, s) : gp_gate<false, GL_GELU>(p, s);
+    case GL_SIGMOID: return backward ? gp_gate<true, GL_SIGMOID>(p, s) : gp_gate<false, GL_SIGMOID>(p, s);
+    default: return backward ? gp_gate<true, GL_RELU>(p, s) : gp_gate<false, GL_RELU>(p, s);
+    }
 }
 
 int hn_launch_gated_linear_pp_products(GlJobs& jobs, hipStream_t s)
