@@ -10,20 +10,20 @@
 
 namespace {
 
-// both projections of TS rows x TS/2 hidden units, and y, or dg and du
-template <typename T, int TS, bool BWD>
-__global__ __launch_bounds__(256) void gl_gate_kernel(GlArgs p)
+// both projections of TI rows x TJ/2 hidden units, and y, or dg and du
+template <typename T, int TI, int TJ, bool BWD>
+__global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int N = TS / 32, G = TS / 16, RP = 256 / G;             // 8-column groups of a row, rows of a pass
-    const long nt = (p.F + TS / 2 - 1) / (TS / 2), mt = (p.M + TS - 1) / TS;
+    constexpr int G = TJ / 16, RP = 256 / G;                          // 8-column groups of a row, rows of a pass
+    const long nt = (p.F + TJ / 2 - 1) / (TJ / 2), mt = (p.M + TI - 1) / TI;
     const long tile = gl_tile_of(blockIdx.x, nt * mt);
-    const long m0 = tile / nt * TS, f0 = tile % nt * (TS / 2);
-    f32x4 acc[N][N];
+    const long m0 = tile / nt * TI, f0 = tile % nt * (TJ / 2);
+    f32x4 acc[TI / 32][TJ / 32];
     const int chunks = (int)((p.K + GlNum<T>::BK - 1) / GlNum<T>::BK);
-    gl_loop<T, TS, GL_KC, GL_DUAL>(lds, acc, p.x, m0, p.w, f0, p.K, chunks, 0, chunks);
+    gl_loop<T, TI, TJ, GL_KC, GL_DUAL>(lds, acc, p.x, m0, p.w, f0, p.K, chunks, 0, chunks);
     float* t = reinterpret_cast<float*>(lds);
-    gl_dump<TS>(t, acc);
+    gl_dump<TI, TJ>(t, acc);
     const int cg = threadIdx.x % G, row0 = threadIdx.x / G;
     const int col = (cg >> 1) * 32 + (cg & 1) * 8;                    // of the gate; the up projection lies 16 columns on
     const long f = f0 + cg * 8, left = p.F - f;
@@ -35,15 +35,15 @@ __global__ __launch_bounds__(256) void gl_gate_kernel(GlArgs p)
         sg[e] = su[e] = 0.f;
     }
 #pragma unroll
-    for (int ps = 0; ps < TS / RP; ++ps) {
+    for (int ps = 0; ps < TI / RP; ++ps) {
         const int row = row0 + ps * RP;
         const long m = m0 + row;
         if (m < p.M && left > 0) {
             float g[8], u[8];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f32x4 tg = *reinterpret_cast<const f32x4*>(t + row * (TS + 4) + col + 4 * h);
-                const f32x4 tu = *reinterpret_cast<const f32x4*>(t + row * (TS + 4) + col + 16 + 4 * h);
+                const f32x4 tg = *reinterpret_cast<const f32x4*>(t + row * (TJ + 4) + col + 4 * h);
+                const f32x4 tu = *reinterpret_cast<const f32x4*>(t + row * (TJ + 4) + col + 16 + 4 * h);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { g[4 * h + e] = tg[e] + bg[4 * h + e]; u[4 * h + e] = tu[e] + bu[4 * h + e]; }
             }
@@ -76,65 +76,71 @@ __global__ __launch_bounds__(256) void gl_gate_kernel(GlArgs p)
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            t[row0 * (TS + 1) + cg * 8 + e] = sg[e];
-            t[row0 * (TS + 1) + TS / 2 + cg * 8 + e] = su[e];
+            t[row0 * (TJ + 1) + cg * 8 + e] = sg[e];
+            t[row0 * (TJ + 1) + TJ / 2 + cg * 8 + e] = su[e];
         }
         __syncthreads();
-        if (threadIdx.x < TS) {
-            const int c = threadIdx.x % (TS / 2), up = threadIdx.x / (TS / 2);
+        if (threadIdx.x < TJ) {
+            const int c = threadIdx.x % (TJ / 2), up = threadIdx.x / (TJ / 2);
             float sum = 0.f;
-            for (int r = 0; r < RP; ++r) sum += t[r * (TS + 1) + up * (TS / 2) + c];
-            if (f0 + c < p.F) p.slab[(m0 / TS) * 2 * p.F + up * p.F + f0 + c] = sum;
+            for (int r = 0; r < RP; ++r) sum += t[r * (TJ + 1) + up * (TJ / 2) + c];
+            if (f0 + c < p.F) p.slab[(m0 / TI) * 2 * p.F + up * p.F + f0 + c] = sum;
         }
     }
 }
 
-template <typename T, int TS>
-__global__ __launch_bounds__(256) void gl_product_kernel(GlJobs all)
+template <typename T, int TI, int TJ>
+__global__ __launch_bounds__(256, 2) void gl_product_kernel(GlJobs all)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int N = TS / 32, G = TS / 8, RP = 256 / G;
+    constexpr int G = TJ / 8, RP = 256 / G;
     int q = 0;
     if (all.n > 1 && (int)blockIdx.x >= all.j[1].first) q = 1;
     if (all.n > 2 && (int)blockIdx.x >= all.j[2].first) q = 2;
     const GlJob& p = all.j[q];
     const long idx = gl_tile_of((long)blockIdx.x - p.first, p.tiles * p.splits);
     const long split = idx / p.tiles, tile = idx % p.tiles;
-    const long i0 = tile / p.tj * TS, j0 = tile % p.tj * TS;
+    const long i0 = tile / p.tj * TI, j0 = tile % p.tj * TJ;
     const int c0 = (int)split * p.run, c1 = c0 + p.run < p.chunks ? c0 + p.run : p.chunks;
-    f32x4 acc[N][N];
-    if (p.a_kr) gl_loop<T, TS, GL_KR, GL_KR>(lds, acc, p.a, i0, p.b, j0, p.K, p.per, c0, c1);
-    else gl_loop<T, TS, GL_KC, GL_KR>(lds, acc, p.a, i0, p.b, j0, p.K, p.per, c0, c1);
+    f32x4 acc[TI / 32][TJ / 32];
+    if (p.a_kr) gl_loop<T, TI, TJ, GL_KR, GL_KR>(lds, acc, p.a, i0, p.b, j0, p.K, p.per, c0, c1);
+    else gl_loop<T, TI, TJ, GL_KC, GL_KR>(lds, acc, p.a, i0, p.b, j0, p.K, p.per, c0, c1);
     float* t = reinterpret_cast<float*>(lds);
-    gl_dump<TS>(t, acc);
+    gl_dump<TI, TJ>(t, acc);
     const int cg = threadIdx.x % G;
     const long j = j0 + cg * 8, left = p.J - j;
     if (left <= 0) return;
     const bool vec = p.J % 8 == 0;                                    // (outputs start on 16 bytes: checked by the host)
-    for (int row = threadIdx.x / G; row < TS; row += RP) {
+    for (int row = threadIdx.x / G; row < TI; row += RP) {
         const long i = i0 + row;
         if (i >= p.I) break;
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = t[row * (TS + 4) + cg * 8 + e];
+        for (int e = 0; e < 8; ++e) x[e] = t[row * (TJ + 4) + cg * 8 + e];
         if (p.splits > 1) gl_store8(p.part + (split * p.I + i) * p.J + j, x, vec, left);
         else gl_store8((T*)p.out + i * p.J + j, x, vec, left);
     }
 }
 
-// the runs of the split products added in order
+// the runs of the split products added up: 64 results a workgroup, its four waves take every fourth run each (in order, eight loads in flight),
+// and their four sums are added in order
 template <typename T>
 __global__ __launch_bounds__(256) void gl_join_kernel(GlJobs all)
 {
-    for (int q = 0; q < all.n; ++q) {
-        const GlJob& p = all.j[q];
-        if (p.splits <= 1) continue;
-        const long n = p.I * p.J;
-        for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
-            float s[1] = {0.f};
-            for (int k = 0; k < p.splits; ++k) s[0] += p.part[k * n + e];
-            seq_store<1>((T*)p.out + e, s);
-        }
+    __shared__ float part[4][64];
+    const GlJob& p = all.j[blockIdx.y];
+    const long n = p.I * p.J, e = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int w = threadIdx.x >> 6;
+    if (p.splits <= 1 || (long)blockIdx.x * 64 >= n) return;
+    float s = 0.f;
+    if (e < n)
+#pragma unroll 8
+        for (int k = w; k < p.splits; k += 4) s += p.part[k * n + e];
+    part[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w == 0 && e < n) {
+        float x[1] = {part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]};
+        seq_store<1>((T*)p.out + e, x);
     }
 }
 
@@ -160,20 +166,30 @@ __global__ __launch_bounds__(256) void gl_pack_kernel(GlPack p)
     }
 }
 
+// the row tiles' column sums added up the same way
 template <typename T>
 __global__ __launch_bounds__(256) void gl_bias_kernel(const float* slab, long tiles, long F, T* dbg, T* dbu)
 {
-    const long c = (long)blockIdx.x * 256 + threadIdx.x;
-    if (c >= 2 * F) return;
-    float s[1] = {0.f};
-    for (long t = 0; t < tiles; ++t) s[0] += slab[t * 2 * F + c];
-    if (c < F) { if (dbg) seq_store<1>(dbg + c, s); }
-    else if (dbu) seq_store<1>(dbu + c - F, s);
+    __shared__ float part[4][64];
+    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int w = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < 2 * F)
+#pragma unroll 8
+        for (long t = w; t < tiles; t += 4) s += slab[t * 2 * F + c];
+    part[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w == 0 && c < 2 * F) {
+        float x[1] = {part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]};
+        if (c < F) { if (dbg) seq_store<1>(dbg + c, x); }
+        else if (dbu) seq_store<1>(dbu + c - F, x);
+    }
 }
 
+constexpr long GL_WIDE = 1L << 20;     // widest K and F: 256 rows of dg | du lie within 32-bit offsets
 int gl_check(int64_t M, int64_t K, int64_t F, int dtype, int act)
 {
-    HN_REQUIRE(M >= 0 && K >= 0 && F >= 0 && M < (1L << 31) && K < (1L << 24) && F < (1L << 24), "hn_gated_linear: bad sizes M=%ld K=%ld F=%ld", (long)M, (long)K,
+    HN_REQUIRE(M >= 0 && K >= 0 && F >= 0 && M < (1L << 31) && K < GL_WIDE && F < GL_WIDE, "hn_gated_linear: bad sizes M=%ld K=%ld F=%ld", (long)M, (long)K,
                (long)F);
     HN_REQUIRE(dtype == SEQ_F32 || dtype == SEQ_BF16, "hn_gated_linear: dtype is 0 (float32) or 1 (bf16)");
     HN_REQUIRE(act >= GL_SILU && act <= GL_RELU, "hn_gated_linear: activation is 0 (silu), 1 (gelu), 2 (sigmoid) or 3 (relu)");
@@ -188,18 +204,42 @@ struct GlIn {
     long ldx, ldg, ldu, M, K, F;
     int size;             // bytes of an element
 };
-// whether the tiles may read a matrix where it lies: rows of whole 16-byte units
-bool gl_aligned(const GlIn& in, const void* p, long ld) { return (size_t)p % 16 == 0 && ld * in.size % 16 == 0 && in.K * in.size % 16 == 0; }
+// whether the tiles may read a matrix where it lies: rows of whole 16-byte units, 256 of them within 32-bit offsets
+bool gl_aligned(const GlIn& in, const void* p, long ld)
+{
+    return (size_t)p % 16 == 0 && ld * in.size % 16 == 0 && in.K * in.size % 16 == 0 && ld * in.size < (1L << 23);
+}
 
 // workspace in order: x and w in whole units where they are not, dgu, column sums, partial products
 struct GlPlan {
-    int ts_gate, ts_prod;
+    int gate, prod;                                   // shapes: 0 64 x 64, 1 128 x 64, 2 128 x 128
     size_t x, wg, wu, dgu, slab, part[3], bytes;      // offsets; 0-size parts share one
     bool pack_x, pack_g, pack_u, pp_gate, pp_prod;
     int splits[3], run[3];
 };
-constexpr long GL_PP_TILES = 192;
 long gl_tiles(long I, long J, int ti, int tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); }
+
+int gl_shape_i(int shape) { return shape == 0 ? 64 : 128; }
+int gl_shape_j(int shape) { return shape == 2 ? 128 : 64; }
+// The gate's tile shape: the one that leaves the fullest of 256 compute units the least to do -- its tiles, times a tile's size, times what a
+// shape costs beyond its size.  bf16 feels the small tile's operand reads (M 2048, K 1024, F 4096: 77 / 50 / 49 us in the order of the shapes;
+// M 512, K 1024, F 2048: 13.8 / 12.2 / 16.5; M 256, K 512, F 1024: 6.0 / 8.2 / 11.4); float32 is bound by its products whatever the shape, and
+// takes the first two alone (M 1999, K 1000, F 1365: 115 / 108).
+int gl_gate_shape(int size, long M, long F)
+{
+    const double more[3] = {1.6, 1.25, 1.0};
+    int best = 0;
+    double least = 0;
+    for (int q = 0; q < (size == 2 ? 3 : 2); ++q) {
+        if (size == 4 && q == 1 && gl_tiles(M, F, 128, 32) < 512) break;      // (two tiles a unit hide each other's waits: M 1000, K 512, F 1000: 21.6 against 23.7)
+        const double cost = (double)((gl_tiles(M, F, gl_shape_i(q), gl_shape_j(q) / 2) + 255) / 256) * (1 << q) * (size == 2 ? more[q] : 1.0);
+        if (q == 0 || cost <= least) { best = q; least = cost; }
+    }
+    return best;
+}
+// The products' shape: 128 x 128 in bf16 where that gives at least 320 tiles (M 16384, K 256, F 2048: products 134 us against 155; below, 64 x 64
+// fills the device better: M 2000, K 1024, F 1365: 49 against 54), else 64 x 64 (float32, M 1999, K 1000, F 1365: 205 against 222)
+int gl_product_shape(int size, long M, long K, long F) { return size == 2 && gl_tiles(M, K, 128, 128) + 2 * gl_tiles(F, K, 128, 128) >= 320 ? 2 : 0; }
 
 GlPlan gl_plan(const GlIn& in, bool backward)
 {
@@ -213,21 +253,25 @@ GlPlan gl_plan(const GlIn& in, bool backward)
     p.x = take(p.pack_x ? (size_t)M * gl_up8(K) * in.size : 0);
     p.wg = take(p.pack_g ? (size_t)F * gl_up8(K) * in.size : 0);
     p.wu = take(p.pack_u ? (size_t)F * gl_up8(K) * in.size : 0);
-    // the ping-pong tiles where they nearly fill the device; their loader's offsets are 32 bits over 256 rows
-    const long most = 1L << 22, ldx = p.pack_x ? gl_up8(K) : in.ldx, ldg = p.pack_g ? gl_up8(K) : in.ldg, ldu = p.pack_u ? gl_up8(K) : in.ldu;
-    const bool pp = in.size == 2 && ldx < most && ldg < most && ldu < most && F < most / 2;
-    p.pp_gate = pp && K >= 128 && gl_tiles(M, F, 256, 128) >= GL_PP_TILES;
-    // the large tile where it still gives every compute unit a workgroup
-    p.ts_gate = gl_tiles(M, F, 128, 64) >= 256 ? 128 : 64;
+    // the ping-pong tiles where they fill three quarters of the device (M 8192, K 256, F 1024, 256 tiles: 15.8 us against 21.5; M 2000, K 1024,
+    // F 1365, 88 tiles: 38 against 25)
+    const long ldg = p.pack_g ? gl_up8(K) : in.ldg, ldu = p.pack_u ? gl_up8(K) : in.ldu;
+    const bool pp = in.size == 2;
+    p.pp_gate = pp && K >= 128 && gl_tiles(M, F, 256, 128) >= 192;
+    p.gate = gl_gate_shape(in.size, M, F);
     if (backward) {
         p.dgu = take((size_t)M * 2 * gl_up8(F) * in.size);
         p.slab = take((size_t)((M + 63) / 64) * 2 * F * 4);
         const long I[3] = {M, F, F}, chunks[3] = {2 * ((F + bk - 1) / bk), (M + bk - 1) / bk, (M + bk - 1) / bk};
-        p.pp_prod = pp && ldg == ldu && M >= 128 && F >= 64 && gl_tiles(M, K, 256, 256) + 2 * gl_tiles(F, K, 256, 256) >= GL_PP_TILES;
-        p.ts_prod = gl_tiles(M, K, 128, 128) + 2 * gl_tiles(F, K, 128, 128) >= 512 ? 128 : 64;
+// the products' ping-pong tiles go out one a compute unit, 2.0 us a chunk: worth it where the longest tile, or all of them over 256
+        // units, end before the smaller tiles would at 600 TFLOP/s (M 8192, K 1024, F 4096: 264 us against 412; M 4096, K 1024, F 2048: 115 against 103)
+        const long cx = 2 * ((F + 63) / 64), cw = (M + 63) / 64, work = gl_tiles(M, K, 256, 256) * cx + 2 * gl_tiles(F, K, 256, 256) * cw;
+        const double longest = (double)(cx > cw ? cx : cw), mean = (double)work / 256;
+        p.pp_prod = pp && ldg == ldu && M >= 128 && F >= 64 && 2.0 * (longest > mean ? longest : mean) < 8.0 * M * K * F / 600e6;
+        p.prod = gl_product_shape(in.size, M, K, F);
         for (int q = 0; q < 3; ++q) {
             // few tiles with a long k axis: runs of at least 4 chunks, as many as bring the product to 256 workgroups
-            const long tiles = gl_tiles(I[q], K, p.ts_prod, p.ts_prod);
+            const long tiles = gl_tiles(I[q], K, gl_shape_i(p.prod), gl_shape_j(p.prod));
             long s = tiles > 0 ? 256 / tiles : 1;
             if (s > chunks[q] / 4) s = chunks[q] / 4;
             if (s < 1 || p.pp_prod) s = 1;
@@ -282,26 +326,34 @@ int gl_big_lds(const void* kern, int bytes, bool (&told)[64])
     return 0;
 }
 
-template <typename T, int TS, bool BWD>
-int gl_gate(const GlArgs& p, hipStream_t s)
+template <typename T, int TI, int TJ, bool BWD>
+int gl_gate_run(const GlArgs& p, hipStream_t s)
 {
-    const long n = gl_tiles(p.M, p.F, TS, TS / 2);
+    const long n = gl_tiles(p.M, p.F, TI, TJ / 2);
     HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear: too many tiles");
     static bool told[64] = {};
-    if (const int rc = gl_big_lds(reinterpret_cast<const void*>(gl_gate_kernel<T, TS, BWD>), gl_lds_bytes<TS>(), told)) return rc;
-    hipLaunchKernelGGL((gl_gate_kernel<T, TS, BWD>), dim3((unsigned)n), dim3(256), gl_lds_bytes<TS>(), s, p);
+    if (const int rc = gl_big_lds(reinterpret_cast<const void*>(gl_gate_kernel<T, TI, TJ, BWD>), gl_lds_bytes<TI, TJ>(), told)) return rc;
+    hipLaunchKernelGGL((gl_gate_kernel<T, TI, TJ, BWD>), dim3((unsigned)n), dim3(256), (gl_lds_bytes<TI, TJ>()), s, p);
     HN_LAUNCH_CHECK();
     return 0;
 }
 
-template <typename T, int TS>
-int gl_products(GlJobs& jobs, hipStream_t s)
+template <typename T, bool BWD>
+int gl_gate(int shape, const GlArgs& p, hipStream_t s)
+{
+    if constexpr (sizeof(T) == 2)
+        if (shape == 2) return gl_gate_run<T, 128, 128, BWD>(p, s);
+    return shape == 0 ? gl_gate_run<T, 64, 64, BWD>(p, s) : gl_gate_run<T, 128, 64, BWD>(p, s);
+}
+
+template <typename T, int TI, int TJ>
+int gl_products_run(GlJobs& jobs, hipStream_t s)
 {
     long n = 0, most = 0;
     for (int q = 0; q < jobs.n; ++q) {
         GlJob& j = jobs.j[q];
-        j.tj = (j.J + TS - 1) / TS;
-        j.tiles = gl_tiles(j.I, j.J, TS, TS);
+        j.tj = (j.J + TJ - 1) / TJ;
+        j.tiles = gl_tiles(j.I, j.J, TI, TJ);
         j.first = (int)n;
         n += j.tiles * j.splits;
         HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear_bwd: too many tiles");
@@ -309,16 +361,23 @@ int gl_products(GlJobs& jobs, hipStream_t s)
     }
     if (n == 0) return 0;
     static bool told[64] = {};
-    if (const int rc = gl_big_lds(reinterpret_cast<const void*>(gl_product_kernel<T, TS>), gl_lds_bytes<TS>(), told)) return rc;
-    hipLaunchKernelGGL((gl_product_kernel<T, TS>), dim3((unsigned)n), dim3(256), gl_lds_bytes<TS>(), s, jobs);
+    if (const int rc = gl_big_lds(reinterpret_cast<const void*>(gl_product_kernel<T, TI, TJ>), gl_lds_bytes<TI, TJ>(), told)) return rc;
+    hipLaunchKernelGGL((gl_product_kernel<T, TI, TJ>), dim3((unsigned)n), dim3(256), (gl_lds_bytes<TI, TJ>()), s, jobs);
     HN_LAUNCH_CHECK();
     if (most) {
-        long g = (most + 255) / 256;
-        if (g > 2048) g = 2048;
-        hipLaunchKernelGGL((gl_join_kernel<T>), dim3((unsigned)g), dim3(256), 0, s, jobs);
+        HN_REQUIRE((most + 63) / 64 <= 0x7fffffffL, "hn_gated_linear_bwd: too many results");
+        hipLaunchKernelGGL((gl_join_kernel<T>), dim3((unsigned)((most + 63) / 64), jobs.n), dim3(256), 0, s, jobs);
         HN_LAUNCH_CHECK();
     }
     return 0;
+}
+
+template <typename T>
+int gl_products(int shape, GlJobs& jobs, hipStream_t s)
+{
+    if constexpr (sizeof(T) == 2)
+        if (shape == 2) return gl_products_run<T, 128, 128>(jobs, s);
+    return gl_products_run<T, 64, 64>(jobs, s);
 }
 
 template <typename T>
@@ -327,7 +386,7 @@ int gl_forward(const GlIn& in, GlArgs p, char* ws, hipStream_t s)
     const GlPlan pl = gl_plan(in, false);
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
     if (pl.pp_gate) return hn_launch_gated_linear_pp_gate(p, false, s);
-    return pl.ts_gate == 128 ? gl_gate<T, 128, false>(p, s) : gl_gate<T, 64, false>(p, s);
+    return gl_gate<T, false>(pl.gate, p, s);
 }
 
 template <typename T>
@@ -335,13 +394,12 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
 {
     const GlPlan pl = gl_plan(in, true);
     const long bk = GlNum<T>::BK, Fp = p.Fp;
-    const int rows = pl.pp_gate ? 128 : pl.ts_gate;                   // of a column-sum tile
+    const int rows = pl.pp_gate ? 128 : gl_shape_i(pl.gate);                 // of a column-sum tile
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
     p.dgu = ws + pl.dgu;
     p.slab = dbg || dbu ? (float*)(ws + pl.slab) : nullptr;
     if (in.M > 0 && in.F > 0)
-        if (const int rc = pl.pp_gate ? hn_launch_gated_linear_pp_gate(p, true, s) : pl.ts_gate == 128 ? gl_gate<T, 128, true>(p, s) : gl_gate<T, 64, true>(p, s))
-            return rc;
+        if (const int rc = pl.pp_gate ? hn_launch_gated_linear_pp_gate(p, true, s) : gl_gate<T, true>(pl.gate, p, s)) return rc;
     GlJobs jobs = {};
     void* outs[3] = {dx, dwg, dwu};
     for (int q = 0; q < 3; ++q) {
@@ -366,9 +424,9 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
         j.splits = pl.splits[q]; j.run = pl.run[q];
         j.part = (float*)(ws + pl.part[q]);
     }
-    if (const int rc = pl.pp_prod ? hn_launch_gated_linear_pp_products(jobs, s) : pl.ts_prod == 128 ? gl_products<T, 128>(jobs, s) : gl_products<T, 64>(jobs, s)) return rc;
+    if (const int rc = pl.pp_prod ? hn_launch_gated_linear_pp_products(jobs, s) : gl_products<T>(pl.prod, jobs, s)) return rc;
     if ((dbg || dbu) && in.F > 0)
-        hipLaunchKernelGGL((gl_bias_kernel<T>), dim3((unsigned)((2 * in.F + 255) / 256)), dim3(256), 0, s, p.slab, (in.M + rows - 1) / rows, in.F, (T*)dbg, (T*)dbu);
+        hipLaunchKernelGGL((gl_bias_kernel<T>), dim3((unsigned)((2 * in.F + 63) / 64)), dim3(256), 0, s, p.slab, (in.M + rows - 1) / rows, in.F, (T*)dbg, (T*)dbu);
     HN_LAUNCH_CHECK();
     return 0;
 }
@@ -383,7 +441,7 @@ GlIn gl_in(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* 
 extern "C" size_t hn_gated_linear_workspace(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, int64_t M,
                                             int64_t K, int64_t F, int dtype, int backward)
 {
-    if (M < 0 || K < 0 || F < 0 || M >= (1L << 31) || K >= (1L << 24) || F >= (1L << 24) || (dtype != SEQ_F32 && dtype != SEQ_BF16)) return 0;
+    if (M < 0 || K < 0 || F < 0 || M >= (1L << 31) || K >= GL_WIDE || F >= GL_WIDE || (dtype != SEQ_F32 && dtype != SEQ_BF16)) return 0;
     return gl_plan(gl_in(x, ldx, w_gate, ld_gate, w_up, ld_up, M, K, F, dtype), backward != 0).bytes;
 }
 

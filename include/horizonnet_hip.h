@@ -448,7 +448,7 @@ int hn_gated_recurrence_step(const void* f, int64_t f_b, const void* v, int64_t 
                              int64_t B, int64_t C, int dtype, void* stream);
 
 /* Gated linear block:  y = act(x w_gate^T + b_gate) * (x w_up^T + b_up),  x [M][K], w [F][K] by their row strides, biases [F] or null,
- * y [M][F] contiguous.  act: 0 silu, 1 gelu (error function), 2 sigmoid, 3 relu.  workspace: hn_gated_linear_workspace() bytes (of the
+ * y [M][F] contiguous, K and F below 2^20.  act: 0 silu, 1 gelu (error function), 2 sigmoid, 3 relu.  workspace: hn_gated_linear_workspace() bytes (of the
  * addresses only the alignment counts), on 16 bytes.
  * hn_gated_linear_bwd: dy [M][F] by its row stride; dx [M][K], dw_* [F][K] on 16 bytes, db_* [F], contiguous, each may be null. */
 size_t hn_gated_linear_workspace(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, int64_t M,

@@ -106,7 +106,8 @@ def test_library_refusals():
     _fails(lin(dtype=-1), "dtype")
     _fails(lin(act=4), "activation")
     _fails(lin(y=None), "null pointer")
-    _fails(lin(K=1 << 24), "bad sizes")
+    _fails(lin(K=1 << 20), "bad sizes")
+    _fails(lin(F=1 << 20), "bad sizes")
     _fails(lib.hn_gated_linear_bwd(one, 8, one, 8, one, 8, None, None, one, 8, one, one, one, None, None, None, 0, 4, 8, 8, 0, 0, None), "workspace too small")
     assert lin(M=0, y=None) == 0
 
