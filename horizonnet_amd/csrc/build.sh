@@ -51,3 +51,15 @@ for q in $PIDS; do wait $q || exit 1; done
 echo "built $(readlink -f $OUT)"
 # an unresolved kernel stub only shows up at dlopen time: fail the build, not the first GPU call
 python3 -c "import ctypes,sys; ctypes.CDLL('$(readlink -f $OUT)')" || { echo "libhorizonnet_hip.so does not load"; exit 1; }
+# the sequence operators' torch side (argument checks, autograd nodes): host code over the library just built
+if [ "$OUT" = ../libhorizonnet_hip.so ]; then
+  EXT=../_sequence_torch.so
+  if [ ! -f $EXT ] || [ sequence_torch.cpp -nt $EXT ] || [ ../../include/horizonnet_hip.h -nt $EXT ] || [ build.sh -nt $EXT ]; then
+    TORCH=$(python3 -c "import os, torch; print(os.path.dirname(torch.__file__))")
+    PYINC=$(python3 -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+    g++ -O2 -std=c++17 -fPIC -shared -Wall -Wno-unused-function -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -DTORCH_EXTENSION_NAME=_sequence_torch -DTORCH_API_INCLUDE_EXTENSION_H \
+      -isystem $TORCH/include -isystem $TORCH/include/torch/csrc/api/include -isystem $PYINC -isystem /opt/rocm/include sequence_torch.cpp -o $EXT \
+      -L.. -lhorizonnet_hip -L$TORCH/lib -ltorch_python -ltorch -ltorch_cpu -ltorch_hip -lc10 -lc10_hip -Wl,-rpath,'$ORIGIN'
+  fi
+  (cd ../.. && python3 -c "import torch; from horizonnet_amd import _sequence_torch") || { echo "_sequence_torch.so does not load"; exit 1; }
+fi
