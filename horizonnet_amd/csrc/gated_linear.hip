@@ -89,6 +89,80 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
     }
 }
 
+// Few rows (M <= 16 NM, one to NM tiles of 16): the weights' bytes are all that counts, so no tile of them goes through LDS.  A workgroup owns 16
+// hidden units; its four waves take a quarter of k each and load the 16 gate rows and 16 up rows straight into fragments, four chunks of 128
+// bytes in flight (16 loads of 16 bytes a lane), x being the other operand; their sums meet in LDS, in order.
+// v_mfma 16 x 16: rows are hidden units, columns rows of x.
+template <typename T, int NM>
+__global__ __launch_bounds__(256) void gl_rows_kernel(GlArgs p)
+{
+    constexpr int BK = GlNum<T>::BK, E = GlNum<T>::E, IN = 4;
+    __shared__ float red[4][2][NM][16][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, kg = lane >> 4;
+    const long f0 = 16L * blockIdx.x;
+    const int chunks = (int)((p.K + BK - 1) / BK), per = (chunks + 3) / 4, c0 = wave * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+    const char* bases[3] = {(const char*)p.w.p[0] + f0 * p.w.ld[0] * (long)sizeof(T), (const char*)p.w.p[1] + f0 * p.w.ld[1] * (long)sizeof(T), (const char*)p.x.p[0]};
+    __amdgpu_buffer_rsrc_t rs[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) rs[q] = __builtin_amdgcn_make_buffer_rsrc((void*)bases[q], 0, 0x7fffffff, 0x00020000);
+    unsigned off[2 + NM];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) off[q] = f0 + l16 < p.F ? (unsigned)l16 * (unsigned)(p.w.ld[q] * (long)sizeof(T)) + 16u * kg : GL_NONE;
+#pragma unroll
+    for (int n = 0; n < NM; ++n) off[2 + n] = 16 * n + l16 < p.M ? (unsigned)(16 * n + l16) * (unsigned)(p.x.ld[0] * (long)sizeof(T)) + 16u * kg : GL_NONE;
+    f32x4 acc[2][NM];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int n = 0; n < NM; ++n) acc[w][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = c0; c < c1; c += IN) {
+        gl_u32x4 r[IN][2][2 + NM];
+#pragma unroll
+        for (int d = 0; d < IN; ++d)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool on = c + d < c1 && (c + d) * BK + (4 * j + kg) * E < p.K;
+#pragma unroll
+                for (int q = 0; q < 2 + NM; ++q)
+                    r[d][j][q] = __builtin_amdgcn_raw_buffer_load_b128(rs[q < 2 ? q : 2], on ? off[q] : GL_NONE, (unsigned)(c + d) * 128u + 64u * j, 0);
+            }
+#pragma unroll
+        for (int d = 0; d < IN; ++d)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int n = 0; n < NM; ++n)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const gl_u32x4 a[1] = {r[d][j][w]}, b[1] = {r[d][j][2 + n]};
+                        f32x4 one[1][1] = {{acc[w][n]}};
+#pragma unroll
+                        for (int m = 0; m < gl_products_of<T, 1, 1>(); ++m) gl_mma<T, 1, 1>(a, b, one, m);
+                        acc[w][n] = one[0][0];
+                    }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int n = 0; n < NM; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) red[wave][w][n][l16][4 * kg + q] = acc[w][n][q];
+    __syncthreads();
+    const int f = threadIdx.x & 15;
+#pragma unroll
+    for (int n = 0; n < NM; ++n) {
+        const int row = threadIdx.x >> 4;
+        const long m = 16 * n + row;
+        if (m >= p.M || f0 + f >= p.F) continue;
+        float g = p.bg ? gl_ld((const T*)p.bg + f0 + f) : 0.f, u = p.bu ? gl_ld((const T*)p.bu + f0 + f) : 0.f, a, slope;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { g += red[w][0][n][row][f]; u += red[w][1][n][row][f]; }
+        gl_act<sizeof(T) == 4>(g, p.act, a, slope);
+        const float y[1] = {a * u};
+        seq_store<1>((T*)p.y + m * p.F + f0 + f, y);
+    }
+}
+
 template <typename T, int TI, int TJ>
 __global__ __launch_bounds__(256, 2) void gl_product_kernel(GlJobs all)
 {
@@ -386,6 +460,13 @@ int gl_forward(const GlIn& in, GlArgs p, char* ws, hipStream_t s)
     const GlPlan pl = gl_plan(in, false);
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
     if (pl.pp_gate) return hn_launch_gated_linear_pp_gate(p, false, s);
+    if (in.M <= 32) {                 // (K 1024, F 4096, bf16 / float32: M 1 5.7 us against 10.6 / 10.5 against 23.0, M 32 7.9 / 10.7 and 15.6 / 23.2)
+        const dim3 grid((unsigned)((in.F + 15) / 16));
+        if (in.M <= 16) hipLaunchKernelGGL((gl_rows_kernel<T, 1>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((gl_rows_kernel<T, 2>), grid, dim3(256), 0, s, p);
+        HN_LAUNCH_CHECK();
+        return 0;
+    }
     return gl_gate<T, false>(pl.gate, p, s);
 }
 

@@ -83,18 +83,18 @@ template <int CL, int VEC>
 __device__ __forceinline__ RecPlace rec_place(const RecArgs& p)
 {
     RecPlace r;
-    long i = blockIdx.x;
-    const long g = i % p.groups; i /= p.groups;
-    const int d = (int)(i % p.dirs); i /= p.dirs;
-    r.b = i % p.B;
-    r.s = (int)(i / p.B);
+    unsigned i = blockIdx.x;              // (the grid has fewer than 2^31 workgroups: 32-bit divisions)
+    const unsigned per = (unsigned)p.groups, q = i / per, g = i - q * per, q2 = p.dirs == 2 ? q >> 1 : q;
+    const int d = (int)(q - q2 * (unsigned)p.dirs);
+    r.s = (int)(q2 / (unsigned)p.B);
+    r.b = q2 - (unsigned)r.s * (unsigned)p.B;
     r.cl = threadIdx.x & (CL - 1);
     r.tl = threadIdx.x / CL;
-    long cd = g * CL * VEC + r.cl * VEC;
+    long cd = (long)g * CL * VEC + r.cl * VEC;
     r.back = (p.reverse != 0) != (d != 0);
     r.live = cd < p.Cd;
     if (r.live && cd > p.Cd - VEC) cd = p.Cd - VEC;   // the last lane's channels end with the row: those that it shares get the same bits twice
-    r.whole = (g + 1) * CL * VEC <= p.Cd;
+    r.whole = (long)(g + 1) * CL * VEC <= p.Cd;
     r.c = (long)d * p.Cd + cd;
     r.bc = r.b * p.C + r.c;
     long len = p.T;
