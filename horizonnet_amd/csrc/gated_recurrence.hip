@@ -27,7 +27,7 @@
 
 namespace {
 
-constexpr int TILE = 128;                 // steps of a tile = steps between two kept states
+constexpr int SHORT = 128, LONG = 256;    // steps of a tile = steps between two kept states
 
 struct RecArgs {
     const void *f, *v, *o, *dy;           // o may be null: y = h
@@ -131,7 +131,7 @@ __device__ __forceinline__ void rec_spans_fold(const float* agg, long BC, long b
 }
 
 // PASS 0: outputs; 1: fold every span to (A, H) only
-template <typename T, int CL, int VEC, int L, int PASS>
+template <typename T, int TILE, int CL, int VEC, int L, int PASS>
 __global__ __launch_bounds__(TILE / L * CL, 2) void gated_recurrence_kernel(RecArgs p)
 {
     constexpr int TL = TILE / L, NW = TL * CL / 64;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(TILE / L * CL, 2) void gated_recurrence_kernel(RecA
 }
 
 // PASS 0: gradients; 1: fold every span to the map of e over it
-template <typename T, int CL, int VEC, int L, int PASS>
+template <typename T, int TILE, int CL, int VEC, int L, int PASS>
 __global__ __launch_bounds__(TILE / L * CL, 2) void gated_recurrence_bwd_kernel(RecArgs p)
 {
     constexpr int TL = TILE / L, NW = TL * CL / 64;
@@ -552,34 +552,44 @@ __global__ __launch_bounds__(256) void gated_recurrence_step_kernel(const T* f, 
     seq_store<VEC>(y + b * C + c, out);
 }
 
-// Spans (and with them the workspace) by the sizes alone: one launch while a sequence has at most 8 tiles or the device is full of sequences
-// and channels, else as many spans as bring the launch to 1024 workgroups, whole tiles each
-void rec_spans(long T, long B, long C, int dirs, int& S, int& span)
+// How a size is cut, by the sizes alone (the states and the workspace go by it).  rows: groups of 64 channels of all sequences.
+//   tiles   128 steps, the last tile's loads beside this one's work; 256 by twice the threads for T 129 .. 512 while they leave the device half
+//           empty (T 256, B 1, C 1024: 6.3 us against 7.7 in float32, 7.2 against 8.4 in bf16)
+//   spans   a lone workgroup takes 2.6 us a tile, 128 of them 3.2 TB/s; a second launch costs 5 us and half as many reads again at 4.6 TB/s.  So longer
+//           sequences are cut while rows < 128, into as many spans as make 1024 workgroups (T 1201, B 1, C 512 float32: 10.8 us against 28.7; T 4096,
+//           B 8, C 512: 73 against 90, bf16 42 against 96), and not beyond (T 1024, B 32, C 512, rows 256: 47.6 us whole against 73 cut)
+struct RecPlan {
+    int tile, S, span;
+};
+RecPlan rec_plan(long T, long B, long C, int dirs)
 {
-    const long tiles = (T + TILE - 1) / TILE, rows = (C / dirs + 63) / 64 * dirs * B;
-    long s = tiles > 8 && rows > 0 ? 1024 / rows : 1;
-    s = s < 1 ? 1 : s > 128 ? 128 : s;
-    if (s > tiles) s = tiles < 1 ? 1 : tiles;
-    span = (int)((tiles + s - 1) / s);
-    if (span < 1) span = 1;
-    S = (int)((tiles + span - 1) / span);
-    if (S < 1) S = 1;
+    RecPlan p;
+    const long rows = (C / dirs + 63) / 64 * dirs * B;
+    p.tile = T > SHORT && T <= 2 * LONG && rows < 256 ? LONG : SHORT;
+    const long tiles = (T + p.tile - 1) / p.tile;
+    long s = T > 2 * LONG && rows < 128 ? 1024 / rows : 1;
+    s = s > 128 ? 128 : s;
+    if (s > tiles) s = tiles;
+    p.span = s < 1 ? 1 : (int)((tiles + s - 1) / s);
+    p.S = tiles < 1 ? 1 : (int)((tiles + p.span - 1) / p.span);
+    return p;
 }
 
-template <typename T, int CL, int VEC, int L, bool BWD>
-int rec_launch(RecArgs p, hipStream_t s)
+template <typename T, int TILE, int CL, int VEC, int L, bool BWD>
+int rec_launch(RecArgs p, const RecPlan& plan, hipStream_t s)
 {
     p.groups = hn_cdiv(p.Cd, CL * VEC);
-    const long rows = (long)p.groups * p.dirs * p.B;
-    rec_spans(p.T, p.B, p.C, p.dirs, p.S, p.span);
-    HN_REQUIRE(rows * p.S <= 0x7fffffffL, "hn_gated_recurrence: too many sequences x channels");
-    const dim3 grid((unsigned)(rows * p.S)), block(TILE / L * CL);
+    p.S = plan.S;
+    p.span = plan.span;
+    const long n = (long)p.groups * p.dirs * p.B * p.S;
+    HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_recurrence: too many sequences x channels");
+    const dim3 grid((unsigned)n), block(TILE / L * CL);
     if constexpr (BWD) {
-        if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, CL, VEC, L, 1>), grid, block, 0, s, p);
-        hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, CL, VEC, L, 0>), grid, block, 0, s, p);
+        if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, TILE, CL, VEC, L, 1>), grid, block, 0, s, p);
+        hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, TILE, CL, VEC, L, 0>), grid, block, 0, s, p);
     } else {
-        if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_kernel<T, CL, VEC, L, 1>), grid, block, 0, s, p);
-        hipLaunchKernelGGL((gated_recurrence_kernel<T, CL, VEC, L, 0>), grid, block, 0, s, p);
+        if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_kernel<T, TILE, CL, VEC, L, 1>), grid, block, 0, s, p);
+        hipLaunchKernelGGL((gated_recurrence_kernel<T, TILE, CL, VEC, L, 0>), grid, block, 0, s, p);
     }
     HN_LAUNCH_CHECK();
     return 0;
@@ -588,11 +598,17 @@ int rec_launch(RecArgs p, hipStream_t s)
 // Four channels a lane, but for rows shorter than that; 128 bytes of a row per workgroup.  8 steps a lane in bf16 (fewer joins an element:
 // 15.4 us against 19.4 forward, 25.4 against 32 backward at T 256, B 32, C 1024), 4 in float32 (16 bytes a load: 16.3 against 21.0 forward, 25.4
 // against 29.2 backward at T 1201, B 7, C 333).
+template <bool BWD, int TILE>
+int rec_dispatch_tile(const RecArgs& p, const RecPlan& plan, int dtype, hipStream_t s)
+{
+    if (p.Cd < 4) return dtype == SEQ_BF16 ? rec_launch<seq_bf16, TILE, 4, 1, 2, BWD>(p, plan, s) : rec_launch<float, TILE, 4, 1, 2, BWD>(p, plan, s);
+    return dtype == SEQ_F32 ? rec_launch<float, TILE, 8, 4, 4, BWD>(p, plan, s) : rec_launch<seq_bf16, TILE, 16, 4, 8, BWD>(p, plan, s);
+}
 template <bool BWD>
 int rec_dispatch(const RecArgs& p, int dtype, hipStream_t s)
 {
-    if (p.Cd < 4) return dtype == SEQ_BF16 ? rec_launch<seq_bf16, 4, 1, 2, BWD>(p, s) : rec_launch<float, 4, 1, 2, BWD>(p, s);
-    return dtype == SEQ_F32 ? rec_launch<float, 8, 4, 4, BWD>(p, s) : rec_launch<seq_bf16, 16, 4, 8, BWD>(p, s);
+    const RecPlan plan = rec_plan(p.T, p.B, p.C, p.dirs);
+    return plan.tile == LONG ? rec_dispatch_tile<BWD, LONG>(p, plan, dtype, s) : rec_dispatch_tile<BWD, SHORT>(p, plan, dtype, s);
 }
 
 int rec_check(long T, long B, long C, int dtype, int direction)
@@ -608,15 +624,14 @@ int rec_check(long T, long B, long C, int dtype, int direction)
 
 extern "C" size_t hn_gated_recurrence_states(int64_t T, int64_t B, int64_t C)
 {
-    return T <= 0 || B <= 0 || C <= 0 ? 0 : (size_t)((T + TILE - 1) / TILE) * B * C;
+    return T <= 0 || B <= 0 || C <= 0 ? 0 : (size_t)((T + SHORT - 1) / SHORT) * B * C;
 }
 
 extern "C" size_t hn_gated_recurrence_workspace(int64_t T, int64_t B, int64_t C, int direction)
 {
     if (T <= 0 || B <= 0 || C <= 0) return 0;
-    int S, span;
-    rec_spans(T, B, C, direction == 2 ? 2 : 1, S, span);
-    return S > 1 ? (size_t)S * 2 * B * C : 0;
+    const RecPlan p = rec_plan(T, B, C, direction == 2 ? 2 : 1);
+    return p.S > 1 ? (size_t)p.S * 2 * B * C : 0;
 }
 
 extern "C" int hn_gated_recurrence(const void* f, int64_t f_t, int64_t f_b, const void* v, int64_t v_t, int64_t v_b, const void* o, int64_t o_t, int64_t o_b,
