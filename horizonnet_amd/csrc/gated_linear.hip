@@ -533,6 +533,7 @@ extern "C" int hn_gated_linear(const void* x, int64_t ldx, const void* w_gate, i
     if (const int rc = gl_check(M, K, F, dtype, act)) return rc;
     if (M == 0 || F == 0) return 0;
     HN_REQUIRE(y && (K == 0 || (x && w_gate && w_up)), "hn_gated_linear: null pointer");
+    HN_REQUIRE(ldx >= 0 && ld_gate >= 0 && ld_up >= 0, "hn_gated_linear: negative row stride");
     const GlIn in = gl_in(x, ldx, w_gate, ld_gate, w_up, ld_up, M, K, F, dtype);
     HN_REQUIRE(workspace_bytes >= gl_plan(in, false).bytes && (workspace || workspace_bytes == 0) && (size_t)workspace % 16 == 0,
                "hn_gated_linear: workspace too small or not aligned to 16 bytes");
@@ -549,6 +550,7 @@ extern "C" int hn_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gat
 {
     if (const int rc = gl_check(M, K, F, dtype, act)) return rc;
     HN_REQUIRE(M == 0 || F == 0 || (dy && (K == 0 || (x && w_gate && w_up))), "hn_gated_linear_bwd: null pointer");
+    HN_REQUIRE(ldx >= 0 && ld_gate >= 0 && ld_up >= 0 && ld_dy >= 0, "hn_gated_linear_bwd: negative row stride");
     const GlIn in = gl_in(x, ldx, w_gate, ld_gate, w_up, ld_up, M, K, F, dtype);
     HN_REQUIRE(workspace_bytes >= gl_plan(in, true).bytes && (workspace || workspace_bytes == 0) && (size_t)workspace % 16 == 0,
                "hn_gated_linear_bwd: workspace too small or not aligned to 16 bytes");

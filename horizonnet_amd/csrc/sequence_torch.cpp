@@ -52,6 +52,8 @@ void check_like(const char* who, const char* name, const Tensor& t, at::IntArray
 // channels next to each other; the other axes as they are
 Tensor rows(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 Tensor whole(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// row stride of a matrix; of a single row any: the one that keeps it aligned
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 int64_t stride_of(const Tensor& t, int axis) { return t.defined() ? t.stride(axis) : 0; }
 // An input that may be missing goes to an autograd node as std::optional: the node takes the defined ones alone as its edges, in order
 typedef std::optional<Tensor> Maybe;
@@ -174,7 +176,6 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& forget, const Tensor& 
 Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Tensor& state, const Maybe& out_gate)
 {
     const char* who = "gated_recurrence_step";
-    const at::AutoGradMode off(false);
     check_main(who, "forget", forget);
     TORCH_CHECK_VALUE(forget.dim() == 2, who, ": forget must be [B, C], got shape ", forget.sizes());
     const auto dev = forget.device();
@@ -183,6 +184,8 @@ Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Te
     if (out_gate) { check_like(who, "out_gate", *out_gate, forget.sizes(), forget.scalar_type(), dev); o = rows(*out_gate); }
     check_like(who, "state", state, forget.sizes(), at::kFloat, dev);
     TORCH_CHECK_VALUE(state.is_contiguous(), who, ": state is updated in place and must be contiguous");
+    TORCH_CHECK(!wants_grad({&forget, &value, &o, &state}), who, " is not differentiable: call it under torch.no_grad() or use gated_recurrence");
+    const at::AutoGradMode off(false);
     const Tensor f = rows(forget), v = rows(value);
     const c10::DeviceGuard guard(dev);
     Tensor y = at::empty(forget.sizes(), f.options());
@@ -199,9 +202,9 @@ Tensor linear_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const
     const c10::DeviceGuard guard(x.device());
     const int64_t M = x.size(0), K = x.size(1), F = wg.size(0);
     Tensor y = at::empty({M, F}, x.options()), ws;
-    const size_t n = hn_gated_linear_workspace(addr(x), x.stride(0), addr(wg), wg.stride(0), addr(wu), wu.stride(0), M, K, F, dtype_of(x), 0);
+    const size_t n = hn_gated_linear_workspace(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), M, K, F, dtype_of(x), 0);
     if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
-    check(hn_gated_linear(addr(x), x.stride(0), addr(wg), wg.stride(0), addr(wu), wu.stride(0), addr(bg), addr(bu), addr(y), addr(ws), n, M, K, F, dtype_of(x),
+    check(hn_gated_linear(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), addr(bg), addr(bu), addr(y), addr(ws), n, M, K, F, dtype_of(x),
                           (int)act, stream_of(x)),
           "hn_gated_linear");
     return y;
@@ -230,10 +233,10 @@ struct Linear : torch::autograd::Function<Linear> {
             if (ctx->needs_input_grad(2)) out[2] = at::empty({F, K}, x.options());
             if (bg.defined() && ctx->needs_input_grad(3)) out[3] = at::empty({F}, x.options());
             if (bu.defined() && ctx->needs_input_grad(bg.defined() ? 4 : 3)) out[4] = at::empty({F}, x.options());
-            const size_t n = hn_gated_linear_workspace(addr(x), x.stride(0), addr(wg), wg.stride(0), addr(wu), wu.stride(0), M, K, F, dtype_of(x), 1);
+            const size_t n = hn_gated_linear_workspace(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), M, K, F, dtype_of(x), 1);
             Tensor ws;
             if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
-            check(hn_gated_linear_bwd(addr(x), x.stride(0), addr(wg), wg.stride(0), addr(wu), wu.stride(0), addr(bg), addr(bu), addr(dy), dy.stride(0), addr(out[0]),
+            check(hn_gated_linear_bwd(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), addr(bg), addr(bu), addr(dy), row_stride(dy), addr(out[0]),
                                       addr(out[1]), addr(out[2]), addr(out[3]), addr(out[4]), addr(ws), n, M, K, F, dtype_of(x),
                                       (int)ctx->saved_data["act"].toInt(), stream_of(x)),
                   "hn_gated_linear_bwd");

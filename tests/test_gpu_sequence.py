@@ -66,6 +66,14 @@ def test_recurrence(T, B, C, direction, name):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("T,B,C,direction", [(128, 1, 8, "reverse"), (129, 1, 8, "forward"), (512, 1, 6, "both"), (513, 1, 8, "reverse"), (640, 2, 6, "both"),
+                                             (2600, 100, 4, "forward"), (1500, 64, 10, "both")])
+def test_recurrence_cuts(T, B, C, direction, name):
+    """Where the tiles and spans of a long sequence begin: their edges, spans of one and of several tiles, all three ways of taking a length."""
+    _rec_check(_rec_case(T, B, C, DT[name]), direction, name)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("T,B,C,gate,h0", [(300, 2, 5, True, True), (33, 1, 1, False, False), (513, 2, 8, False, True), (20, 2, 12, True, False)])
 def test_recurrence_optional_inputs_and_odd_channels(T, B, C, gate, h0, name):
     _rec_check(_rec_case(T, B, C, DT[name], gate, h0), "reverse" if C == 5 else "forward", name)
@@ -314,6 +322,20 @@ def test_linear_shapes_and_some_gradients(name):
     _near("shared dx", got[1], want["dx"].sum(0, keepdim=True), off["dx"].sum(0, keepdim=True) + 8 * half * terms)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_linear_single_rows(name):
+    """One row, one hidden unit, any stride on the axis of length one."""
+    g = torch.Generator().manual_seed(12)
+    x, wg, wu, dy = (_normal(g, *s, dtype=DT[name]) for s in ((1, 40), (3, 40), (3, 40), (1, 3)))
+    want, off = ref.linear(x, wg, wu, None, None, "gelu", dy)
+    for stride in (0, 1, 41, 1 << 40):
+        leaves = [x.to(DEV).as_strided((1, 40), (stride, 1)).detach().requires_grad_(True), wg.to(DEV).requires_grad_(True), wu.to(DEV).requires_grad_(True)]
+        y = hn.gated_linear(*leaves, activation="gelu")
+        _near("y", y, want["y"], off["y"])
+        for n, t in zip(("dx", "dwg", "dwu"), torch.autograd.grad(y, leaves, dy.to(DEV))):
+            _near(n, t, want[n], off[n])
+
+
 def test_linear_nothing_to_do():
     for dtype in DT.values():
         for M, K, F in ((0, 8, 8), (3, 0, 8), (3, 8, 0)):
@@ -409,6 +431,9 @@ def test_refusals():
         (ValueError, lambda: hn.gated_recurrence(x, x, lengths=torch.ones(3, device=DEV).int())),
         (ValueError, lambda: hn.gated_recurrence_step(x, x, x)), (ValueError, lambda: hn.gated_recurrence_step(x[0], x[0], b[0])),
         (ValueError, lambda: hn.gated_recurrence_step(x[0], x[0], torch.zeros(8, 2, device=DEV).t())),
+        (RuntimeError, lambda: hn.gated_recurrence_step(x[0], x[0], torch.zeros(2, 8, device=DEV, requires_grad=True))),
+        (RuntimeError, lambda: hn.gated_recurrence_step(x[0].clone().requires_grad_(True), x[0], torch.zeros(2, 8, device=DEV))),
+        (TypeError, lambda: hn.gated_linear(x, None, None)), (TypeError, lambda: hn.dropout(x, "half", 1)), (TypeError, lambda: hn.gated_recurrence(x, 3)),
         (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 7, device=DEV), torch.zeros(3, 7, device=DEV))),
         (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(4, 8, device=DEV))),
         (ValueError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(3, 8, device=DEV), activation="tanh")),
