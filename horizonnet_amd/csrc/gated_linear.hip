@@ -196,25 +196,34 @@ __global__ __launch_bounds__(256, 2) void gl_product_kernel(GlJobs all)
     }
 }
 
-// the runs of the split products added up: 64 results a workgroup, its four waves take every fourth run each (in order, eight loads in flight),
-// and their four sums are added in order
+// What is left of the backward pass, one launch: the runs of the split products added up, and the row tiles' column sums of dg | du (the last
+// plane of the grid).  64 results a workgroup; its four waves take every fourth summand each (in order, eight loads in flight), and their four
+// sums are added in order.
+struct GlFinish {
+    const float* part[4];     // [n][count]
+    long n[4], count[4];      // summands, results
+    void* out[4];
+    void* up;                 // the column sums' second half
+};
 template <typename T>
-__global__ __launch_bounds__(256) void gl_join_kernel(GlJobs all)
+__global__ __launch_bounds__(256) void gl_finish_kernel(GlFinish p, int bias)
 {
     __shared__ float part[4][64];
-    const GlJob& p = all.j[blockIdx.y];
-    const long n = p.I * p.J, e = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int w = threadIdx.x >> 6;
-    if (p.splits <= 1 || (long)blockIdx.x * 64 >= n) return;
+    const int q = blockIdx.y, w = threadIdx.x >> 6;
+    const long count = p.count[q], e = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    if ((long)blockIdx.x * 64 >= count) return;
     float s = 0.f;
-    if (e < n)
+    if (e < count)
 #pragma unroll 8
-        for (int k = w; k < p.splits; k += 4) s += p.part[k * n + e];
+        for (long k = w; k < p.n[q]; k += 4) s += p.part[q][k * count + e];
     part[w][threadIdx.x & 63] = s;
     __syncthreads();
-    if (w == 0 && e < n) {
-        float x[1] = {part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]};
-        seq_store<1>((T*)p.out + e, x);
+    if (w == 0 && e < count) {
+        const float x[1] = {part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]};
+        T* out = (T*)p.out[q];
+        long at = e;
+        if (q == bias && e >= count / 2) { out = (T*)p.up; at = e - count / 2; }
+        if (out) seq_store<1>(out + at, x);
     }
 }
 
@@ -237,26 +246,6 @@ __global__ __launch_bounds__(256) void gl_pack_kernel(GlPack p)
             gl_load8((const T*)p.src[q] + row * p.ld[q] + k, x, false, p.K - k);
             gl_store8((T*)p.dst[q] + row * p.Kp + k, x, true, 8);
         }
-    }
-}
-
-// the row tiles' column sums added up the same way
-template <typename T>
-__global__ __launch_bounds__(256) void gl_bias_kernel(const float* slab, long tiles, long F, T* dbg, T* dbu)
-{
-    __shared__ float part[4][64];
-    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int w = threadIdx.x >> 6;
-    float s = 0.f;
-    if (c < 2 * F)
-#pragma unroll 8
-        for (long t = w; t < tiles; t += 4) s += slab[t * 2 * F + c];
-    part[w][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (w == 0 && c < 2 * F) {
-        float x[1] = {part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]};
-        if (c < F) { if (dbg) seq_store<1>(dbg + c, x); }
-        else if (dbu) seq_store<1>(dbu + c - F, x);
     }
 }
 
@@ -423,7 +412,7 @@ int gl_gate(int shape, const GlArgs& p, hipStream_t s)
 template <typename T, int TI, int TJ>
 int gl_products_run(GlJobs& jobs, hipStream_t s)
 {
-    long n = 0, most = 0;
+    long n = 0;
     for (int q = 0; q < jobs.n; ++q) {
         GlJob& j = jobs.j[q];
         j.tj = (j.J + TJ - 1) / TJ;
@@ -431,18 +420,12 @@ int gl_products_run(GlJobs& jobs, hipStream_t s)
         j.first = (int)n;
         n += j.tiles * j.splits;
         HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear_bwd: too many tiles");
-        if (j.splits > 1 && j.I * j.J > most) most = j.I * j.J;
     }
     if (n == 0) return 0;
     static bool told[64] = {};
     if (const int rc = gl_big_lds(reinterpret_cast<const void*>(gl_product_kernel<T, TI, TJ>), gl_lds_bytes<TI, TJ>(), told)) return rc;
     hipLaunchKernelGGL((gl_product_kernel<T, TI, TJ>), dim3((unsigned)n), dim3(256), (gl_lds_bytes<TI, TJ>()), s, jobs);
     HN_LAUNCH_CHECK();
-    if (most) {
-        HN_REQUIRE((most + 63) / 64 <= 0x7fffffffL, "hn_gated_linear_bwd: too many results");
-        hipLaunchKernelGGL((gl_join_kernel<T>), dim3((unsigned)((most + 63) / 64), jobs.n), dim3(256), 0, s, jobs);
-        HN_LAUNCH_CHECK();
-    }
     return 0;
 }
 
@@ -506,8 +489,24 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
         j.part = (float*)(ws + pl.part[q]);
     }
     if (const int rc = pl.pp_prod ? hn_launch_gated_linear_pp_products(jobs, s) : gl_products<T>(pl.prod, jobs, s)) return rc;
-    if ((dbg || dbu) && in.F > 0)
-        hipLaunchKernelGGL((gl_bias_kernel<T>), dim3((unsigned)((2 * in.F + 63) / 64)), dim3(256), 0, s, p.slab, (in.M + rows - 1) / rows, in.F, (T*)dbg, (T*)dbu);
+    GlFinish fin = {};
+    int planes = 0, bias = -1;
+    long most = 0;
+    auto add = [&](const float* part, long n, long count, void* out) {
+        fin.part[planes] = part; fin.n[planes] = n; fin.count[planes] = count; fin.out[planes] = out;
+        most = count > most ? count : most;
+        return planes++;
+    };
+    for (int q = 0; q < jobs.n; ++q)
+        if (jobs.j[q].splits > 1) add(jobs.j[q].part, jobs.j[q].splits, jobs.j[q].I * jobs.j[q].J, jobs.j[q].out);
+    if ((dbg || dbu) && in.F > 0) {
+        bias = add(p.slab, (in.M + rows - 1) / rows, 2 * in.F, dbg);
+        fin.up = dbu;
+    }
+    if (planes) {
+        HN_REQUIRE((most + 63) / 64 <= 0x7fffffffL, "hn_gated_linear_bwd: too many results");
+        hipLaunchKernelGGL((gl_finish_kernel<T>), dim3((unsigned)((most + 63) / 64), planes), dim3(256), 0, s, fin, bias);
+    }
     HN_LAUNCH_CHECK();
     return 0;
 }
