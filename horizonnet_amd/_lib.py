@@ -99,8 +99,9 @@ SIGNATURES = {
                                      _i64, _i64, _i64, _i, _i, _vp]),
     "hn_gated_recurrence_step": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i, _vp]),
     "hn_gated_linear_workspace": (_sz, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i, _i]),
-    "hn_gated_linear": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
-    "hn_gated_linear_bwd": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
+    "hn_gated_linear_kept": (_sz, [_i64, _i64, _i64, _i]),
+    "hn_gated_linear": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
+    "hn_gated_linear_bwd": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i, _i, _vp]),
     "hn_dropout": (_i, [_vp, _vp, _vp, _i64, _i, _f, _c.c_uint64, _vp, _vp]),
 }
 

@@ -18,6 +18,7 @@ struct GlArgs {
     const void *bg, *bu, *dy;
     long ldd;
     void *y, *dgu;        // dgu: dg | du, rows of 2 Fp
+    float* kept;          // g | u as the forward pass formed them, rows of 2 Fp, or null
     float* slab;          // [row tiles][2F] column sums of dg | du, or null
     long M, K, F, Fp;
     int act, dy_vec, y_vec;

@@ -2,8 +2,11 @@
 //
 //     g = x Wg^T + bg     u = x Wu^T + bu     y = act(g) * u            x [M][K], W [F][K] (the layout of a Linear's weight), y [M][F]
 //
-// g and u are never stored.  The backward pass forms them again tile by tile and writes what the products need,
+// The backward pass needs g and u once more, and writes what its products need,
 //     dg = dy u act'(g)      du = dy act(g)        (one [M][2F] buffer, dg | du, in the inputs' type)
+// In bf16 it forms g and u again tile by tile (rounded to bf16 they would cost the gradients a third of their precision, and in float32 their way
+// through memory takes as long as the products: M 8192, K 1024, F 4096, 165 us against 150).  In float32, whose products run at a tenth of that
+// rate, the forward pass keeps them (K >= 128; M 1999, K 1000, F 1365: 110 us of products against 22 of traffic).
 // then  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x;  the bias gradients are column sums of the unrounded dg, du, per row tile into a
 // slab that a last pass adds in order (no atomics: the same bits every time).
 #include "gated_linear_tile.h"
@@ -48,6 +51,10 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
                 for (int e = 0; e < 4; ++e) { g[4 * h + e] = tg[e] + bg[4 * h + e]; u[4 * h + e] = tu[e] + bu[4 * h + e]; }
             }
             if constexpr (!BWD) {
+                if (sizeof(T) == 4 && p.kept) {
+                    gl_store8(p.kept + m * 2 * p.Fp + f, g, true, 8);
+                    gl_store8(p.kept + m * 2 * p.Fp + p.Fp + f, u, true, 8);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float a, slope;
@@ -85,6 +92,51 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
             float sum = 0.f;
             for (int r = 0; r < RP; ++r) sum += t[r * (TJ + 1) + up * (TJ / 2) + c];
             if (f0 + c < p.F) p.slab[(m0 / TI) * 2 * p.F + up * p.F + f0 + c] = sum;
+        }
+    }
+}
+
+// dg | du from the kept g | u: 64 rows x 64 hidden units a workgroup, bound by its 5 float32 transfers an element
+template <typename T>
+__global__ __launch_bounds__(256) void gl_slope_kernel(GlArgs p)
+{
+    __shared__ float sums[32][129];
+    const long nt = (p.F + 63) / 64, m0 = blockIdx.x / nt * 64, f0 = blockIdx.x % nt * 64;
+    const int cg = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+    const long f = f0 + cg * 8, left = p.F - f;
+    float sg[8], su[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
+#pragma unroll
+    for (int ps = 0; ps < 2; ++ps) {
+        const long m = m0 + row0 + 32 * ps;
+        if (m < p.M && left > 0) {
+            float g[8], u[8], d[8];
+            gl_load8(p.kept + m * 2 * p.Fp + f, g, left >= 8, left);
+            gl_load8(p.kept + m * 2 * p.Fp + p.Fp + f, u, left >= 8, left);
+            gl_load8((const T*)p.dy + m * p.ldd + f, d, p.dy_vec, left);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {                             // (past F: all three are 0)
+                float a, slope;
+                gl_act<sizeof(T) == 4>(g[e], p.act, a, slope);
+                g[e] = d[e] * u[e] * slope;
+                u[e] = d[e] * a;
+                sg[e] += g[e];
+                su[e] += u[e];
+            }
+            gl_store8((T*)p.dgu + m * 2 * p.Fp + f, g, true, 8);
+            gl_store8((T*)p.dgu + m * 2 * p.Fp + p.Fp + f, u, true, 8);
+        }
+    }
+    if (p.slab) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { sums[row0][cg * 8 + e] = sg[e]; sums[row0][64 + cg * 8 + e] = su[e]; }
+        __syncthreads();
+        if (threadIdx.x < 128) {
+            const int c = threadIdx.x & 63, up = threadIdx.x >> 6;
+            float sum = 0.f;
+            for (int r = 0; r < 32; ++r) sum += sums[r][threadIdx.x];
+            if (f0 + c < p.F) p.slab[m0 / 64 * 2 * p.F + up * p.F + f0 + c] = sum;
         }
     }
 }
@@ -157,6 +209,10 @@ __global__ __launch_bounds__(256) void gl_rows_kernel(GlArgs p)
         float g = p.bg ? gl_ld((const T*)p.bg + f0 + f) : 0.f, u = p.bu ? gl_ld((const T*)p.bu + f0 + f) : 0.f, a, slope;
 #pragma unroll
         for (int w = 0; w < 4; ++w) { g += red[w][0][n][row][f]; u += red[w][1][n][row][f]; }
+        if (sizeof(T) == 4 && p.kept) {
+            p.kept[m * 2 * p.Fp + f0 + f] = g;
+            p.kept[m * 2 * p.Fp + p.Fp + f0 + f] = u;
+        }
         gl_act<sizeof(T) == 4>(g, p.act, a, slope);
         const float y[1] = {a * u};
         seq_store<1>((T*)p.y + m * p.F + f0 + f, y);
@@ -458,11 +514,16 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
 {
     const GlPlan pl = gl_plan(in, true);
     const long bk = GlNum<T>::BK, Fp = p.Fp;
-    const int rows = pl.pp_gate ? 128 : gl_shape_i(pl.gate);                 // of a column-sum tile
+    const int rows = p.kept ? 64 : pl.pp_gate ? 128 : gl_shape_i(pl.gate);                 // of a column-sum tile
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
     p.dgu = ws + pl.dgu;
     p.slab = dbg || dbu ? (float*)(ws + pl.slab) : nullptr;
-    if (in.M > 0 && in.F > 0)
+    if (in.M > 0 && in.F > 0 && p.kept) {
+        const long n = gl_tiles(in.M, in.F, 64, 64);
+        HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear_bwd: too many tiles");
+        hipLaunchKernelGGL((gl_slope_kernel<T>), dim3((unsigned)n), dim3(256), 0, s, p);
+        HN_LAUNCH_CHECK();
+    } else if (in.M > 0 && in.F > 0)
         if (const int rc = pl.pp_gate ? hn_launch_gated_linear_pp_gate(p, true, s) : gl_gate<T, true>(pl.gate, p, s)) return rc;
     GlJobs jobs = {};
     void* outs[3] = {dx, dwg, dwu};
@@ -525,9 +586,14 @@ extern "C" size_t hn_gated_linear_workspace(const void* x, int64_t ldx, const vo
     return gl_plan(gl_in(x, ldx, w_gate, ld_gate, w_up, ld_up, M, K, F, dtype), backward != 0).bytes;
 }
 
+extern "C" size_t hn_gated_linear_kept(int64_t M, int64_t K, int64_t F, int dtype)
+{
+    return dtype == SEQ_F32 && K >= 128 && M > 0 && F > 0 && M < (1L << 31) && F < GL_WIDE ? (size_t)M * 2 * gl_up8(F) : 0;
+}
+
 extern "C" int hn_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,
-                               const void* b_up, void* y, void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act,
-                               void* stream)
+                               const void* b_up, void* y, float* kept, void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F,
+                               int dtype, int act, void* stream)
 {
     if (const int rc = gl_check(M, K, F, dtype, act)) return rc;
     if (M == 0 || F == 0) return 0;
@@ -537,14 +603,15 @@ extern "C" int hn_gated_linear(const void* x, int64_t ldx, const void* w_gate, i
     HN_REQUIRE(workspace_bytes >= gl_plan(in, false).bytes && (workspace || workspace_bytes == 0) && (size_t)workspace % 16 == 0,
                "hn_gated_linear: workspace too small or not aligned to 16 bytes");
     GlArgs p = {};
-    p.bg = b_gate; p.bu = b_up; p.y = y;
+    HN_REQUIRE(!kept || (hn_gated_linear_kept(M, K, F, dtype) && (size_t)kept % 16 == 0), "hn_gated_linear: kept is null where hn_gated_linear_kept is 0, else on 16 bytes");
+    p.bg = b_gate; p.bu = b_up; p.y = y; p.kept = kept;
     p.M = M; p.K = K; p.F = F; p.Fp = gl_up8(F); p.act = act;
     p.y_vec = (size_t)y % 16 == 0 && F * in.size % 16 == 0;
     return dtype == SEQ_BF16 ? gl_forward<seq_bf16>(in, p, (char*)workspace, (hipStream_t)stream) : gl_forward<float>(in, p, (char*)workspace, (hipStream_t)stream);
 }
 
 extern "C" int hn_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,
-                                   const void* b_up, const void* dy, int64_t ld_dy, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
+                                   const void* b_up, const void* dy, int64_t ld_dy, const float* kept, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
                                    void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act, void* stream)
 {
     if (const int rc = gl_check(M, K, F, dtype, act)) return rc;
@@ -555,7 +622,8 @@ extern "C" int hn_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gat
                "hn_gated_linear_bwd: workspace too small or not aligned to 16 bytes");
     HN_REQUIRE((size_t)dx % 16 == 0 && (size_t)dw_gate % 16 == 0 && (size_t)dw_up % 16 == 0, "hn_gated_linear_bwd: dx, dw_gate and dw_up start on 16 bytes");
     GlArgs p = {};
-    p.bg = b_gate; p.bu = b_up; p.dy = dy; p.ldd = ld_dy;
+    HN_REQUIRE(!kept || (hn_gated_linear_kept(M, K, F, dtype) && (size_t)kept % 16 == 0), "hn_gated_linear_bwd: kept is null where hn_gated_linear_kept is 0, else on 16 bytes");
+    p.bg = b_gate; p.bu = b_up; p.dy = dy; p.ldd = ld_dy; p.kept = const_cast<float*>(kept);
     p.M = M; p.K = K; p.F = F; p.Fp = gl_up8(F); p.act = act;
     p.dy_vec = (size_t)dy % 16 == 0 && ld_dy * in.size % 16 == 0;
     return dtype == SEQ_BF16 ? gl_backward<seq_bf16>(in, p, (char*)workspace, dx, dw_gate, dw_up, db_gate, db_up, (hipStream_t)stream)

@@ -197,14 +197,17 @@ Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Te
 }
 
 // ---- gated linear block ----
-Tensor linear_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& bg, const Tensor& bu, int64_t act)
+Tensor linear_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& bg, const Tensor& bu, int64_t act, Tensor* kept)
 {
     const c10::DeviceGuard guard(x.device());
     const int64_t M = x.size(0), K = x.size(1), F = wg.size(0);
     Tensor y = at::empty({M, F}, x.options()), ws;
     const size_t n = hn_gated_linear_workspace(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), M, K, F, dtype_of(x), 0);
     if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
-    check(hn_gated_linear(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), addr(bg), addr(bu), addr(y), addr(ws), n, M, K, F, dtype_of(x),
+    if (kept)
+        if (const size_t floats = hn_gated_linear_kept(M, K, F, dtype_of(x))) *kept = at::empty({(int64_t)floats}, x.options().dtype(at::kFloat));
+    check(hn_gated_linear(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), addr(bg), addr(bu), addr(y),
+                          kept ? addr<float>(*kept) : nullptr, addr(ws), n, M, K, F, dtype_of(x),
                           (int)act, stream_of(x)),
           "hn_gated_linear");
     return y;
@@ -214,14 +217,16 @@ struct Linear : torch::autograd::Function<Linear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Maybe& bg_, const Maybe& bu_, int64_t act)
     {
         const Tensor bg = open(bg_), bu = open(bu_);
-        ctx->save_for_backward({x, wg, wu, bg, bu});
+        Tensor kept;
+        const Tensor y = linear_forward(x, wg, wu, bg, bu, act, &kept);
+        ctx->save_for_backward({x, wg, wu, bg, bu, kept});
         ctx->saved_data["act"] = act;
-        return linear_forward(x, wg, wu, bg, bu, act);
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4];
+        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4], &kept = saved[5];
         const c10::DeviceGuard guard(x.device());
         const int64_t M = x.size(0), K = x.size(1), F = wg.size(0);
         variable_list out(6);
@@ -236,7 +241,8 @@ struct Linear : torch::autograd::Function<Linear> {
             const size_t n = hn_gated_linear_workspace(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), M, K, F, dtype_of(x), 1);
             Tensor ws;
             if (n) ws = at::empty({(int64_t)n}, x.options().dtype(at::kByte));
-            check(hn_gated_linear_bwd(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), addr(bg), addr(bu), addr(dy), row_stride(dy), addr(out[0]),
+            check(hn_gated_linear_bwd(addr(x), row_stride(x), addr(wg), row_stride(wg), addr(wu), row_stride(wu), addr(bg), addr(bu), addr(dy), row_stride(dy),
+                                      addr<float>(kept), addr(out[0]),
                                       addr(out[1]), addr(out[2]), addr(out[3]), addr(out[4]), addr(ws), n, M, K, F, dtype_of(x),
                                       (int)ctx->saved_data["act"].toInt(), stream_of(x)),
                   "hn_gated_linear_bwd");
@@ -265,7 +271,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
     const Tensor x2 = rows(x.dim() == 2 ? x : x.reshape({M, K})), wg = rows(w_gate), wu = rows(w_up);
-    const Tensor y = wants_grad({&x2, &wg, &wu, &bg, &bu}) ? Linear::apply(x2, wg, wu, maybe(bg), maybe(bu), act) : linear_forward(x2, wg, wu, bg, bu, act);
+    const Tensor y = wants_grad({&x2, &wg, &wu, &bg, &bu}) ? Linear::apply(x2, wg, wu, maybe(bg), maybe(bu), act) : linear_forward(x2, wg, wu, bg, bu, act, nullptr);
     if (x.dim() == 2) return y;
     auto shape = x.sizes().vec();
     shape.back() = F;

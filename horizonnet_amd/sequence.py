@@ -47,8 +47,8 @@ def gated_recurrence_step(forget, value, state, out_gate=None):
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)`` in one kernel.  x ``[..., K]``, weights ``[F, K]`` (the layout of
     ``nn.Linear.weight``), biases ``[F]`` or None, each by itself; activation "silu", "gelu" (error function), "sigmoid" or "relu".  Products and
-    activations run in float32 and the result ``[..., F]`` is rounded once to the inputs' type.  The backward pass forms the projections again
-    instead of keeping them: only the inputs stay in memory between the passes."""
+    activations run in float32 and the result ``[..., F]`` is rounded once to the inputs' type.  In bfloat16 the backward pass forms the
+    projections again and only the inputs stay in memory between the passes; in float32 (K >= 128) both projections are kept."""
     return (_native or _load()).gated_linear(x, w_gate, w_up, b_gate, b_up, activation)
 
 

@@ -449,16 +449,18 @@ int hn_gated_recurrence_step(const void* f, int64_t f_b, const void* v, int64_t 
 
 /* Gated linear block:  y = act(x w_gate^T + b_gate) * (x w_up^T + b_up),  x [M][K], w [F][K] by their row strides, biases [F] or null,
  * y [M][F] contiguous, K and F below 2^20.  act: 0 silu, 1 gelu (error function), 2 sigmoid, 3 relu.  workspace: hn_gated_linear_workspace() bytes (of the
- * addresses only the alignment counts), on 16 bytes.
+ * addresses only the alignment counts), on 16 bytes.  kept: hn_gated_linear_kept() floats on 16 bytes that the forward call fills for its
+ * backward call (which forms the projections again without them), or null.
  * hn_gated_linear_bwd: dy [M][F] by its row stride; dx [M][K], dw_* [F][K] on 16 bytes, db_* [F], contiguous, each may be null. */
 size_t hn_gated_linear_workspace(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, int64_t M,
                                  int64_t K, int64_t F, int dtype, int backward);
+size_t hn_gated_linear_kept(int64_t M, int64_t K, int64_t F, int dtype);
 int hn_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,
-                    const void* b_up, void* y, void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act,
-                    void* stream);
+                    const void* b_up, void* y, float* kept, void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype,
+                    int act, void* stream);
 int hn_gated_linear_bwd(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,
-                        const void* b_up, const void* dy, int64_t ld_dy, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
-                        void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act, void* stream);
+                        const void* b_up, const void* dy, int64_t ld_dy, const float* kept, void* dx, void* dw_gate, void* dw_up, void* db_gate,
+                        void* db_up, void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t F, int dtype, int act, void* stream);
 
 /* Dropout:  y[i] = residual[i] + (keep(i) ? x[i] / (1 - p) : 0), keep(i) = the generator's 32 bits at (seed, i) >= p 2^32: the generator of
  * the training step (hn_train_forward's mask behind LSTM layer l is that of seed' = 2 seed + 1 + l).  residual may be null; seed_dev, if not

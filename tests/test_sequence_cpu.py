@@ -100,8 +100,8 @@ def test_library_refusals():
     _fails(lib.hn_gated_recurrence_step(one, 8, one, 8, None, 0, None, one, 2, 8, 0, None), "null pointer")
     _fails(lib.hn_gated_recurrence_step(one, 8, one, 8, None, 0, one, one, 2, 8, 7, None), "dtype")
 
-    def lin(M=4, K=8, F=8, dtype=0, act=0, y=one, ld=8):
-        return lib.hn_gated_linear(one, ld, one, 8, one, 8, None, None, y, None, 0, M, K, F, dtype, act, None)
+    def lin(M=4, K=8, F=8, dtype=0, act=0, y=one, ld=8, kept=None):
+        return lib.hn_gated_linear(one, ld, one, 8, one, 8, None, None, y, kept, None, 0, M, K, F, dtype, act, None)
 
     _fails(lin(dtype=-1), "dtype")
     _fails(lin(act=4), "activation")
@@ -109,7 +109,9 @@ def test_library_refusals():
     _fails(lin(ld=-8), "negative row stride")
     _fails(lin(K=1 << 20), "bad sizes")
     _fails(lin(F=1 << 20), "bad sizes")
-    _fails(lib.hn_gated_linear_bwd(one, 8, one, 8, one, 8, None, None, one, 8, one, one, one, None, None, None, 0, 4, 8, 8, 0, 0, None), "workspace too small")
+    _fails(lin(kept=one), "kept")                             # K < 128: nothing is kept
+    _fails(lib.hn_gated_linear_bwd(one, 8, one, 8, one, 8, None, None, one, 8, None, one, one, one, None, None, None, 0, 4, 8, 8, 0, 0, None), "workspace too small")
+    assert lib.hn_gated_linear_kept(4, 128, 12, 0) == 4 * 2 * 16 and lib.hn_gated_linear_kept(4, 128, 12, 1) == 0
     assert lin(M=0, y=None) == 0
 
     for p in (1.0, -0.1, float("nan")):
