@@ -134,4 +134,16 @@ __device__ __forceinline__ long gl_tile_of(long bid, long n)
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
 }
 
+// the same for a grid of mt x nt tiles, in bands of GL_BAND rows of tiles walked column by column: the tiles that an XCD works on at a time then
+// need GL_BAND row operands and a few column operands, not one row's and all columns'
+// (bands of 4 against 1, bf16 forward at M 16384, K 1024, F 4096: 249.5 us against 266.6; 8: 248.9)
+constexpr long GL_BAND = 4;
+__device__ __forceinline__ void gl_tile_at(long bid, long mt, long nt, long& row, long& col)
+{
+    const long t = gl_tile_of(bid, mt * nt), band = t / (GL_BAND * nt), first = band * GL_BAND, rest = t - first * nt;
+    const long rows = mt - first < GL_BAND ? mt - first : GL_BAND;
+    col = rest / rows;
+    row = first + rest - col * rows;
+}
+
 }  // namespace

@@ -20,8 +20,9 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int G = TJ / 16, RP = 256 / G;                          // 8-column groups of a row, rows of a pass
     const long nt = (p.F + TJ / 2 - 1) / (TJ / 2), mt = (p.M + TI - 1) / TI;
-    const long tile = gl_tile_of(blockIdx.x, nt * mt);
-    const long m0 = tile / nt * TI, f0 = tile % nt * (TJ / 2);
+    long row_tile, col_tile;
+    gl_tile_at(blockIdx.x, mt, nt, row_tile, col_tile);
+    const long m0 = row_tile * TI, f0 = col_tile * (TJ / 2);
     f32x4 acc[TI / 32][TJ / 32];
     const int chunks = (int)((p.K + GlNum<T>::BK - 1) / GlNum<T>::BK);
     gl_loop<T, TI, TJ, GL_KC, GL_DUAL>(lds, acc, p.x, m0, p.w, f0, p.K, chunks, 0, chunks);

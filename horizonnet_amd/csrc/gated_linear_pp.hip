@@ -281,9 +281,10 @@ struct GpGate {
     __device__ __forceinline__ bool tile(int vb, GpTile& t) const
     {
         if (vb >= total) return false;
-        const int tile = (int)gl_tile_of(vb, total), mt = tile / nt;
-        t.i0 = 256L * __builtin_amdgcn_readfirstlane(mt);
-        t.j0 = 128L * __builtin_amdgcn_readfirstlane(tile - mt * nt);
+        long row, col;
+        gl_tile_at(vb, total / nt, nt, row, col);
+        t.i0 = 256L * __builtin_amdgcn_readfirstlane((int)row);
+        t.j0 = 128L * __builtin_amdgcn_readfirstlane((int)col);
         t.chunks = chunks;
         return true;
     }
