@@ -98,7 +98,6 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
 }
 
 // dg | du from the kept g | u: 64 rows x 64 hidden units a workgroup, bound by its 5 float32 transfers an element
-template <typename T>
 __global__ __launch_bounds__(256) void gl_slope_kernel(GlArgs p)
 {
     __shared__ float sums[32][129];
@@ -113,20 +112,20 @@ __global__ __launch_bounds__(256) void gl_slope_kernel(GlArgs p)
         const long m = m0 + row0 + 32 * ps;
         if (m < p.M && left > 0) {
             float g[8], u[8], d[8];
-            gl_load8(p.kept + m * 2 * p.Fp + f, g, left >= 8, left);
-            gl_load8(p.kept + m * 2 * p.Fp + p.Fp + f, u, left >= 8, left);
-            gl_load8((const T*)p.dy + m * p.ldd + f, d, p.dy_vec, left);
+            gl_load8((const float*)p.kept + m * 2 * p.Fp + f, g, left >= 8, left);
+            gl_load8((const float*)p.kept + m * 2 * p.Fp + p.Fp + f, u, left >= 8, left);
+            gl_load8((const float*)p.dy + m * p.ldd + f, d, p.dy_vec, left);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {                             // (past F: all three are 0)
                 float a, slope;
-                gl_act<sizeof(T) == 4>(g[e], p.act, a, slope);
+                gl_act<true>(g[e], p.act, a, slope);
                 g[e] = d[e] * u[e] * slope;
                 u[e] = d[e] * a;
                 sg[e] += g[e];
                 su[e] += u[e];
             }
-            gl_store8((T*)p.dgu + m * 2 * p.Fp + f, g, true, 8);
-            gl_store8((T*)p.dgu + m * 2 * p.Fp + p.Fp + f, u, true, 8);
+            gl_store8((float*)p.dgu + m * 2 * p.Fp + f, g, true, 8);
+            gl_store8((float*)p.dgu + m * 2 * p.Fp + p.Fp + f, u, true, 8);
         }
     }
     if (p.slab) {
@@ -383,7 +382,7 @@ GlPlan gl_plan(const GlIn& in, bool backward)
         p.dgu = take((size_t)M * 2 * gl_up8(F) * in.size);
         p.slab = take((size_t)((M + 63) / 64) * 2 * F * 4);
         const long I[3] = {M, F, F}, chunks[3] = {2 * ((F + bk - 1) / bk), (M + bk - 1) / bk, (M + bk - 1) / bk};
-// the products' ping-pong tiles go out one a compute unit, 2.0 us a chunk: worth it where the longest tile, or all of them over 256
+        // the products' ping-pong tiles go out one a compute unit, 2.0 us a chunk: worth it where the longest tile, or all of them over 256
         // units, end before the smaller tiles would at 600 TFLOP/s (M 8192, K 1024, F 4096: 264 us against 412; M 4096, K 1024, F 2048: 115 against 103)
         const long cx = 2 * ((F + 63) / 64), cw = (M + 63) / 64, work = gl_tiles(M, K, 256, 256) * cx + 2 * gl_tiles(F, K, 256, 256) * cw;
         const double longest = (double)(cx > cw ? cx : cw), mean = (double)work / 256;
@@ -499,7 +498,6 @@ int gl_forward(const GlIn& in, GlArgs p, char* ws, hipStream_t s)
 {
     const GlPlan pl = gl_plan(in, false);
     if (const int rc = gl_prepare<T>(in, pl, ws, p.x, p.w, s)) return rc;
-    if (pl.pp_gate) return hn_launch_gated_linear_pp_gate(p, false, s);
     if (in.M <= 32) {                 // (K 1024, F 4096, bf16 / float32: M 1 5.7 us against 10.6 / 10.5 against 23.0, M 32 7.9 / 10.7 and 15.6 / 23.2)
         const dim3 grid((unsigned)((in.F + 15) / 16));
         if (in.M <= 16) hipLaunchKernelGGL((gl_rows_kernel<T, 1>), grid, dim3(256), 0, s, p);
@@ -507,6 +505,7 @@ int gl_forward(const GlIn& in, GlArgs p, char* ws, hipStream_t s)
         HN_LAUNCH_CHECK();
         return 0;
     }
+    if (pl.pp_gate) return hn_launch_gated_linear_pp_gate(p, false, s);
     return gl_gate<T, false>(pl.gate, p, s);
 }
 
@@ -522,7 +521,7 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
     if (in.M > 0 && in.F > 0 && p.kept) {
         const long n = gl_tiles(in.M, in.F, 64, 64);
         HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear_bwd: too many tiles");
-        hipLaunchKernelGGL((gl_slope_kernel<T>), dim3((unsigned)n), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(gl_slope_kernel, dim3((unsigned)n), dim3(256), 0, s, p);
         HN_LAUNCH_CHECK();
     } else if (in.M > 0 && in.F > 0)
         if (const int rc = pl.pp_gate ? hn_launch_gated_linear_pp_gate(p, true, s) : gl_gate<T, true>(pl.gate, p, s)) return rc;

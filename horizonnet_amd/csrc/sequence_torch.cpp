@@ -325,9 +325,9 @@ Tensor dropout(const Tensor& x_, double p, const py::object& seed_, const Maybe&
         TORCH_CHECK_VALUE(seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x_.device(), who, ": a seed tensor must be one int64 on ",
                           x_.device(), ", got ", seed.sizes(), " ", seed.scalar_type(), " on ", seed.device());
     } else {
-        TORCH_CHECK_VALUE(PyLong_Check(seed_.ptr()) && !PyBool_Check(seed_.ptr()), who, ": seed must be an int in 0 .. 2**64 - 1 or an int64 tensor");
-        number = PyLong_AsUnsignedLongLong(seed_.ptr());
-        if (PyErr_Occurred()) {
+        const py::object whole = PyBool_Check(seed_.ptr()) ? py::object() : py::reinterpret_steal<py::object>(PyNumber_Index(seed_.ptr()));
+        if (whole) number = PyLong_AsUnsignedLongLong(whole.ptr());
+        if (!whole || PyErr_Occurred()) {
             PyErr_Clear();
             TORCH_CHECK_VALUE(false, who, ": seed must be an int in 0 .. 2**64 - 1 or an int64 tensor");
         }

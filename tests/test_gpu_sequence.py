@@ -1,5 +1,6 @@
 """Sequence operators on the device against the 64-bit oracle, whose bounds come from running error analysis (oracle/sequence_ref.py): a
 result may be off by what float32 arithmetic can add and by half a step of the type that it is stored in."""
+import numpy as np
 import pytest
 import torch
 
@@ -258,7 +259,7 @@ def test_linear_sizes(M, K, F, name):
 
 
 @pytest.mark.parametrize("M,K,F,bias,act", [(2048, 128, 4096, 0, "silu"), (4100, 200, 1544, 3, "gelu"), (3000, 1032, 2050, 3, "sigmoid"), (12345, 130, 520, 1, "relu"),
-                                            (600, 1024, 8200, 2, "silu"), (9000, 1096, 1000, 0, "silu")])
+                                            (600, 1024, 8200, 2, "silu"), (9000, 1096, 1000, 0, "silu"), (20, 128, 30000, 3, "silu")])
 def test_linear_large(M, K, F, bias, act):
     """Sizes that take the large tiles, whole and ragged ones: checked against float64 on the device, at every element."""
     g = torch.Generator(device=DEV).manual_seed(M)
@@ -403,6 +404,7 @@ def test_dropout_views():
     assert torch.equal(hn.dropout(x.transpose(0, 2), 0.3, 11), hn.dropout(x.transpose(0, 2).contiguous(), 0.3, 11))
     assert torch.equal(hn.dropout(x[1:, 1:, 1:], 0.3, 11), hn.dropout(x[1:, 1:, 1:].contiguous(), 0.3, 11))
     flat = x.reshape(-1)
+    assert torch.equal(hn.dropout(x, 0.3, np.uint64(2 ** 63 + 5)), hn.dropout(x, 0.3, 2 ** 63 + 5))
     part = flat[1:1001]                                       # contiguous, at an odd offset
     assert torch.equal(hn.dropout(part, 0.3, 11, residual=flat[3:1003]), hn.dropout(part.clone(), 0.3, 11, residual=flat[3:1003].clone()))
 
@@ -442,7 +444,7 @@ def test_refusals():
         (ValueError, lambda: hn.gated_linear(x, torch.zeros(8, device=DEV), torch.zeros(8, device=DEV))),
         (RuntimeError, lambda: hn.gated_linear(x, torch.zeros(3, 8, device=DEV), torch.zeros(3, 8))),
         (ValueError, lambda: hn.dropout(x, 1.0, 1)), (ValueError, lambda: hn.dropout(x, -0.1, 1)), (ValueError, lambda: hn.dropout(x, float("nan"), 1)),
-        (ValueError, lambda: hn.dropout(x, 0.5, -1)), (ValueError, lambda: hn.dropout(x, 0.5, 1.5)), (ValueError, lambda: hn.dropout(x, 0.5, 1 << 64)),
+        (ValueError, lambda: hn.dropout(x, 0.5, True)), (ValueError, lambda: hn.dropout(x, 0.5, None)), (ValueError, lambda: hn.dropout(x, 0.5, -1)), (ValueError, lambda: hn.dropout(x, 0.5, 1.5)), (ValueError, lambda: hn.dropout(x, 0.5, 1 << 64)),
         (ValueError, lambda: hn.dropout(x, 0.5, torch.ones(2, dtype=torch.int64, device=DEV))), (ValueError, lambda: hn.dropout(x, 0.5, torch.ones(1, dtype=torch.int64))),
         (ValueError, lambda: hn.dropout(x, 0.5, 1, residual=x[0])), (ValueError, lambda: hn.dropout(x, 0.5, 1, residual=b)),
         (ValueError, lambda: hn.dropout(x.half(), 0.5, 1)),
