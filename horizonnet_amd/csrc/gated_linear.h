@@ -52,7 +52,7 @@ __device__ __forceinline__ void gl_act(float z, int act, float& a, float& slope)
 {
     if (act == GL_RELU) {
         a = z > 0.f ? z : (z != z ? z : 0.f);
-        slope = z > 0.f ? 1.f : 0.f;
+        slope = z <= 0.f ? 0.f : 1.f;
     } else if (act == GL_GELU) {
         const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
         a = z * cdf;

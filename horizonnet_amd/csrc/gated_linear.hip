@@ -588,7 +588,7 @@ extern "C" size_t hn_gated_linear_workspace(const void* x, int64_t ldx, const vo
 
 extern "C" size_t hn_gated_linear_kept(int64_t M, int64_t K, int64_t F, int dtype)
 {
-    return dtype == SEQ_F32 && K >= 128 && M > 0 && F > 0 && M < (1L << 31) && F < GL_WIDE ? (size_t)M * 2 * gl_up8(F) : 0;
+    return dtype == SEQ_F32 && K >= 128 && K < GL_WIDE && M > 0 && F > 0 && M < (1L << 31) && F < GL_WIDE ? (size_t)M * 2 * gl_up8(F) : 0;
 }
 
 extern "C" int hn_gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, const void* b_gate,

@@ -629,7 +629,7 @@ extern "C" size_t hn_gated_recurrence_states(int64_t T, int64_t B, int64_t C)
 
 extern "C" size_t hn_gated_recurrence_workspace(int64_t T, int64_t B, int64_t C, int direction)
 {
-    if (T <= 0 || B <= 0 || C <= 0) return 0;
+    if (T <= 0 || B <= 0 || C <= 0 || T >= (1L << 31) || B >= (1L << 31) || C >= (1L << 30) || (direction == 2 && C % 2)) return 0;      // (sizes that the calls refuse)
     const RecPlan p = rec_plan(T, B, C, direction == 2 ? 2 : 1);
     return p.S > 1 ? (size_t)p.S * 2 * B * C : 0;
 }

@@ -120,3 +120,14 @@ def test_library_refusals():
     _fails(lib.hn_dropout(one, None, one, 4, 3, 0.5, 1, None, None), "dtype")
     _fails(lib.hn_dropout(one, None, one, -1, 0, 0.5, 1, None, None), "n=-1")
     assert lib.hn_dropout(None, None, None, 0, 0, 0.5, 1, None, None) == 0
+
+
+def test_workspace_of_refused_sizes():
+    """The size functions answer 0 for what the calls refuse (one channel in both directions and steps past 2^31 divided by zero)."""
+    lib = _lib.load()
+    for T, B, C, direction in ((1000, 1, 1, 2), (1000, 3, 7, 2), (1 << 46, 1, 8, 0), (1000, 1 << 33, 8, 0), (1000, 1, 1 << 40, 1), (0, 1, 8, 0), (-5, 1, 8, 0)):
+        assert lib.hn_gated_recurrence_workspace(T, B, C, direction) == 0
+    assert lib.hn_gated_recurrence_workspace(5000, 2, 8, 0) > 0
+    for M, K, F, dtype in ((1 << 31, 8, 8, 0), (4, 1 << 20, 8, 0), (4, 8, 1 << 20, 1), (-1, 8, 8, 0), (4, 8, 8, 2)):
+        assert lib.hn_gated_linear_workspace(256, 8, 256, 8, 256, 8, M, K, F, dtype, 1) == 0
+        assert lib.hn_gated_linear_kept(M, K, F, dtype) == 0
