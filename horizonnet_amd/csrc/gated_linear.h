@@ -1,4 +1,4 @@
-// What the two families of kernels of the gated linear block share: operands, jobs, the activation (gated_linear.hip: 64 / 128 tiles for every
+// What the two families of kernels of the gated linear block share: operands, jobs, the activation (gated_linear.hip: 32 to 128 wide tiles for every
 // size and type; gated_linear_pp.hip: 256 x 256 ping-pong tiles for large bf16 sizes).
 #pragma once
 #include "seq_common.h"

@@ -18,7 +18,7 @@ template <typename T, int TI, int TJ, bool BWD>
 __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int G = TJ / 16, RP = 256 / G;                          // 8-column groups of a row, rows of a pass
+    constexpr int G = TJ / 16, RP = 256 / G < TI ? 256 / G : TI;      // 8-column groups of a row, rows of a pass
     const long nt = (p.F + TJ / 2 - 1) / (TJ / 2), mt = (p.M + TI - 1) / TI;
     long row_tile, col_tile;
     gl_tile_at(blockIdx.x, mt, nt, row_tile, col_tile);
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
     for (int ps = 0; ps < TI / RP; ++ps) {
         const int row = row0 + ps * RP;
         const long m = m0 + row;
-        if (m < p.M && left > 0) {
+        if (m < p.M && left > 0 && (RP * G == 256 || row < TI)) {
             float g[8], u[8];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -83,10 +83,11 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
     if (BWD && p.slab) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            t[row0 * (TJ + 1) + cg * 8 + e] = sg[e];
-            t[row0 * (TJ + 1) + TJ / 2 + cg * 8 + e] = su[e];
-        }
+        for (int e = 0; e < 8; ++e)
+            if (RP * G == 256 || row0 < RP) {
+                t[row0 * (TJ + 1) + cg * 8 + e] = sg[e];
+                t[row0 * (TJ + 1) + TJ / 2 + cg * 8 + e] = su[e];
+            }
         __syncthreads();
         if (threadIdx.x < TJ) {
             const int c = threadIdx.x % (TJ / 2), up = threadIdx.x / (TJ / 2);
@@ -331,28 +332,34 @@ bool gl_aligned(const GlIn& in, const void* p, long ld)
 
 // workspace in order: x and w in whole units where they are not, dgu, column sums, partial products
 struct GlPlan {
-    int gate, prod;                                   // shapes: 0 64 x 64, 1 128 x 64, 2 128 x 128
+    int gate, prod;                                   // shapes
     size_t x, wg, wu, dgu, slab, part[3], bytes;      // offsets; 0-size parts share one
     bool pack_x, pack_g, pack_u, pp_gate, pp_prod;
     int splits[3], run[3];
 };
 long gl_tiles(long I, long J, int ti, int tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); }
 
-int gl_shape_i(int shape) { return shape == 0 ? 64 : 128; }
-int gl_shape_j(int shape) { return shape == 2 ? 128 : 64; }
+// 0 64 x 64, 1 128 x 64, 2 128 x 128 (bf16 alone), 3 64 x 32, 4 32 x 32 (float32 alone)
+int gl_shape_i(int shape) { return shape == 4 ? 32 : shape == 0 || shape == 3 ? 64 : 128; }
+int gl_shape_j(int shape) { return shape == 2 ? 128 : shape >= 3 ? 32 : 64; }
 // The gate's tile shape: the one that leaves the fullest of 256 compute units the least to do -- its tiles, times a tile's size, times what a
-// shape costs beyond its size.  bf16 feels the small tile's operand reads (M 2048, K 1024, F 4096: 77 / 50 / 49 us in the order of the shapes;
-// M 512, K 1024, F 2048: 13.8 / 12.2 / 16.5; M 256, K 512, F 1024: 6.0 / 8.2 / 11.4); float32 is bound by its products whatever the shape, and
-// takes the first two alone (M 1999, K 1000, F 1365: 115 / 108).
+// shape costs beyond its size.
+//   bf16     feels the small tile's operand reads (M 2048, K 1024, F 4096: 77 / 50 / 49 us in the order of the shapes; M 512, K 1024, F 2048: 13.8 /
+//            12.2 / 16.5; M 256, K 512, F 1024: 6.0 / 8.2 / 11.4, and 5.8 by 64 x 32)
+//   float32  is bound by its products, whose time goes with a unit's tiles alone: the small ones where the larger leave units empty, in the first
+//            round or the last (32 x 32 / 64 x 32 / 64 x 64: M 256, K 512, F 512: 7.7 / 9.7 / 13.6; M 512, K 1024, F 1365: 31.9 / 30.8 / 38.2; M 2048,
+//            K 1024, F 4096: 300 / 273 / 266, and 255 by 128 x 64), 128 x 64 where it gives two tiles a unit, which hide each other's waits
 int gl_gate_shape(int size, long M, long F)
 {
-    const double more[3] = {1.6, 1.25, 1.0};
+    static const struct { int shape; double cost; } bf16[3] = {{0, 1.6}, {1, 2.5}, {2, 4.0}}, f32[4] = {{4, 0.28}, {3, 0.525}, {0, 1.0}, {1, 2.0}};
     int best = 0;
     double least = 0;
-    for (int q = 0; q < (size == 2 ? 3 : 2); ++q) {
-        if (size == 4 && q == 1 && gl_tiles(M, F, 128, 32) < 512) break;      // (two tiles a unit hide each other's waits: M 1000, K 512, F 1000: 21.6 against 23.7)
-        const double cost = (double)((gl_tiles(M, F, gl_shape_i(q), gl_shape_j(q) / 2) + 255) / 256) * (1 << q) * (size == 2 ? more[q] : 1.0);
-        if (q == 0 || cost <= least) { best = q; least = cost; }
+    for (int q = 0; q < (size == 2 ? 3 : 4); ++q) {
+        const int shape = size == 2 ? bf16[q].shape : f32[q].shape;
+        const long tiles = gl_tiles(M, F, gl_shape_i(shape), gl_shape_j(shape) / 2);
+        if (size == 4 && shape == 1 && tiles < 512) break;                    // (M 1000, K 512, F 1000: 21.6 by 64 x 64 against 23.7)
+        const double cost = (double)((tiles + 255) / 256) * (size == 2 ? bf16[q].cost : f32[q].cost);
+        if (q == 0 || cost <= least) { best = shape; least = cost; }
     }
     return best;
 }
@@ -380,7 +387,7 @@ GlPlan gl_plan(const GlIn& in, bool backward)
     p.gate = gl_gate_shape(in.size, M, F);
     if (backward) {
         p.dgu = take((size_t)M * 2 * gl_up8(F) * in.size);
-        p.slab = take((size_t)((M + 63) / 64) * 2 * F * 4);
+        p.slab = take((size_t)((M + 31) / 32) * 2 * F * 4);
         const long I[3] = {M, F, F}, chunks[3] = {2 * ((F + bk - 1) / bk), (M + bk - 1) / bk, (M + bk - 1) / bk};
         // the products' ping-pong tiles go out one a compute unit, 2.0 us a chunk: worth it where the longest tile, or all of them over 256
         // units, end before the smaller tiles would at 600 TFLOP/s (M 8192, K 1024, F 4096: 264 us against 412; M 4096, K 1024, F 2048: 115 against 103)
@@ -462,6 +469,10 @@ int gl_gate(int shape, const GlArgs& p, hipStream_t s)
 {
     if constexpr (sizeof(T) == 2)
         if (shape == 2) return gl_gate_run<T, 128, 128, BWD>(p, s);
+    if constexpr (sizeof(T) == 4) {
+        if (shape == 3) return gl_gate_run<T, 64, 32, BWD>(p, s);
+        if (shape == 4) return gl_gate_run<T, 32, 32, BWD>(p, s);
+    }
     return shape == 0 ? gl_gate_run<T, 64, 64, BWD>(p, s) : gl_gate_run<T, 128, 64, BWD>(p, s);
 }
 

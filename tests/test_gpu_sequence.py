@@ -263,6 +263,15 @@ def test_linear_sizes(M, K, F, name):
     _lin_check(M, K, F, name, "silu", 0)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("K", [40, 133])
+@pytest.mark.parametrize("M,F", [(250, 500), (250, 1020), (510, 1000), (2040, 1020)])
+def test_linear_tile_shapes(M, F, K, name):
+    """One size for each tile shape of the float32 projections (32 x 32, 64 x 32, 64 x 64, 128 x 64), where the backward pass forms them again
+    and where they were kept."""
+    _lin_check(M, K, F, name, "silu", 3)
+
+
 @pytest.mark.parametrize("M,K,F,bias,act", [(2048, 128, 4096, 0, "silu"), (4100, 200, 1544, 3, "gelu"), (3000, 1032, 2050, 3, "sigmoid"), (12345, 130, 520, 1, "relu"),
                                             (600, 1024, 8200, 2, "silu"), (9000, 1096, 1000, 0, "silu"), (20, 128, 30000, 3, "silu")])
 def test_linear_large(M, K, F, bias, act):
