@@ -6,7 +6,7 @@
 // affine, h -> A h + H, and two runs join as (A1, H1) then (A2, H2) = (A1 A2, A2 H1 + H2): time is parallel.
 //
 // A workgroup owns CL * VEC channels of one sequence (128 bytes of a row: whole cache lines) and walks its time in tiles of 128 steps (256 where
-// few workgroups have a short sequence): TL time lanes of L consecutive steps each, all of a tile's loads in flight at once and the next tile's
+// few workgroups have a short sequence, 32 or 64 where it is shorter): TL time lanes of L consecutive steps each, all of a tile's loads in flight at once and the next tile's
 // behind them.  Each lane folds its steps to (A, H) in registers, a wave joins its lanes by shuffles, the waves meet in LDS once per tile, and
 // every lane runs its steps again from registers with its true incoming state: each input is read from memory once.  What bounds it is HBM (4
 // tensors forward, 7 backward), with the two gates' exponentials and reciprocals close behind.  bf16, T 256, B 32, C 1024: 15.4 us forward (67 MB,
@@ -28,7 +28,7 @@
 
 namespace {
 
-constexpr int SHORT = 128, LONG = 256;    // steps of a tile = steps between two kept states
+constexpr int TINY = 32, SMALL = 64, SHORT = 128, LONG = 256;    // steps of a tile = steps between two kept states
 
 struct RecArgs {
     const void *f, *v, *o, *dy;           // o may be null: y = h
@@ -555,7 +555,8 @@ __global__ __launch_bounds__(256) void gated_recurrence_step_kernel(const T* f, 
 
 // How a size is cut, by the sizes alone (the states and the workspace go by it).  rows: groups of 64 channels of all sequences.
 //   tiles   128 steps, the last tile's loads beside this one's work; 256 by twice the threads for T 129 .. 512 while they leave the device half
-//           empty (T 256, B 1, C 1024: 6.3 us against 7.7 in float32, 7.2 against 8.4 in bf16)
+//           empty (T 256, B 1, C 1024: 6.3 us against 7.7 in float32, 7.2 against 8.4 in bf16); 32 or 64 for sequences no longer than that, whose
+//           other time lanes would idle (float32 T 8, B 300, C 512: 15.4 us against 46.9; T 64, B 64, C 1024: 16.8 against 24.0)
 //   spans   a lone workgroup takes 2.6 us a tile, 128 of them 3.2 TB/s; a second launch costs 5 us and half as many reads again at 4.6 TB/s.  So longer
 //           sequences are cut while rows < 128, into as many spans as make 1024 workgroups (T 1201, B 1, C 512 float32: 10.8 us against 28.7; T 4096,
 //           B 8, C 512: 73 against 90, bf16 42 against 96), and not beyond (T 1024, B 32, C 512, rows 256: 47.6 us whole against 73 cut)
@@ -566,7 +567,7 @@ RecPlan rec_plan(long T, long B, long C, int dirs)
 {
     RecPlan p;
     const long rows = (C / dirs + 63) / 64 * dirs * B;
-    p.tile = T > SHORT && T <= 2 * LONG && rows < 256 ? LONG : SHORT;
+    p.tile = T <= TINY ? TINY : T <= SMALL ? SMALL : T > SHORT && T <= 2 * LONG && rows < 256 ? LONG : SHORT;
     const long tiles = (T + p.tile - 1) / p.tile;
     long s = T > 2 * LONG && rows < 128 ? 1024 / rows : 1;
     s = s > 128 ? 128 : s;
@@ -586,29 +587,39 @@ int rec_launch(RecArgs p, const RecPlan& plan, hipStream_t s)
     HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_recurrence: too many sequences x channels");
     const dim3 grid((unsigned)n), block(TILE / L * CL);
     if constexpr (BWD) {
-        if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, TILE, CL, VEC, L, 1>), grid, block, 0, s, p);
+        if constexpr (TILE == SHORT)              // (the other tiles are never cut into spans)
+            if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, TILE, CL, VEC, L, 1>), grid, block, 0, s, p);
         hipLaunchKernelGGL((gated_recurrence_bwd_kernel<T, TILE, CL, VEC, L, 0>), grid, block, 0, s, p);
     } else {
-        if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_kernel<T, TILE, CL, VEC, L, 1>), grid, block, 0, s, p);
+        if constexpr (TILE == SHORT)
+            if (p.S > 1) hipLaunchKernelGGL((gated_recurrence_kernel<T, TILE, CL, VEC, L, 1>), grid, block, 0, s, p);
         hipLaunchKernelGGL((gated_recurrence_kernel<T, TILE, CL, VEC, L, 0>), grid, block, 0, s, p);
     }
     HN_LAUNCH_CHECK();
     return 0;
 }
 
-// Four channels a lane, but for rows shorter than that; 128 bytes of a row per workgroup.  8 steps a lane in bf16 (fewer joins an element:
-// 15.4 us against 19.4 forward, 25.4 against 32 backward at T 256, B 32, C 1024), 4 in float32 (16 bytes a load: 16.3 against 21.0 forward, 25.4
-// against 29.2 backward at T 1201, B 7, C 333).
+// Four channels a lane and 128 bytes of a row per workgroup where the device is full: 8 steps a lane in bf16 (fewer joins an element: 15.4 us against
+// 19.4 forward, 25.4 against 32 backward at T 256, B 32, C 1024), 4 in float32 (16 bytes a load: 16.3 against 21.0 forward, 25.4 against 29.2 backward
+// at T 1201, B 7, C 333).  While all workgroups are resident at once, 8 waves a compute unit, the time is a lane's own chain, and less work a lane is
+// faster: one channel a lane (T 256, B 1, C 1024, forward / backward: float32 4.5 / 5.9 us against 6.2 / 9.0, bf16 4.4 / 5.7 against 7.1 / 10.4; past
+// that bound it loses: T 256, B 4 13.1 against 6.7), then, in bf16, half the steps (T 256, B 4: 5.7 / 8.2 against 7.4 / 11.0; T 256, B 15: 14.3
+// against 8.3).  Rows of fewer than four channels take one a lane always.
 template <bool BWD, int TILE>
 int rec_dispatch_tile(const RecArgs& p, const RecPlan& plan, int dtype, hipStream_t s)
 {
-    if (p.Cd < 4) return dtype == SEQ_BF16 ? rec_launch<seq_bf16, TILE, 4, 1, 2, BWD>(p, plan, s) : rec_launch<float, TILE, 4, 1, 2, BWD>(p, plan, s);
-    return dtype == SEQ_F32 ? rec_launch<float, TILE, 8, 4, 4, BWD>(p, plan, s) : rec_launch<seq_bf16, TILE, 16, 4, 8, BWD>(p, plan, s);
+    auto resident = [&](int channels) { return (double)hn_cdiv(p.Cd, channels) * p.dirs * p.B * plan.S * (TILE / 4 * 8) <= 256 * 512; };
+    const bool bf16 = dtype == SEQ_BF16;
+    if (p.Cd < 4 || resident(8)) return bf16 ? rec_launch<seq_bf16, TILE, 8, 1, 4, BWD>(p, plan, s) : rec_launch<float, TILE, 8, 1, 4, BWD>(p, plan, s);
+    if (!bf16) return rec_launch<float, TILE, 8, 4, 4, BWD>(p, plan, s);
+    return resident(32) ? rec_launch<seq_bf16, TILE, 8, 4, 4, BWD>(p, plan, s) : rec_launch<seq_bf16, TILE, 16, 4, 8, BWD>(p, plan, s);
 }
 template <bool BWD>
 int rec_dispatch(const RecArgs& p, int dtype, hipStream_t s)
 {
     const RecPlan plan = rec_plan(p.T, p.B, p.C, p.dirs);
+    if (plan.tile == TINY) return rec_dispatch_tile<BWD, TINY>(p, plan, dtype, s);
+    if (plan.tile == SMALL) return rec_dispatch_tile<BWD, SMALL>(p, plan, dtype, s);
     return plan.tile == LONG ? rec_dispatch_tile<BWD, LONG>(p, plan, dtype, s) : rec_dispatch_tile<BWD, SHORT>(p, plan, dtype, s);
 }
 

@@ -80,6 +80,16 @@ def test_recurrence_cuts(T, B, C, direction, name):
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("T,B,C,direction", [(1, 50, 420, "both"), (31, 70, 1000, "reverse"), (32, 20, 36, "both"), (33, 40, 260, "forward"), (50, 150, 260, "forward"),
+                                             (64, 35, 1001, "reverse"), (64, 5, 30, "both"), (65, 5, 900, "both"), (90, 17, 1001, "forward"), (260, 9, 1000, "reverse"),
+                                             (300, 3, 700, "both"), (5, 3000, 3, "forward")])
+def test_recurrence_widths(T, B, C, direction, name):
+    """One, four and eight channels or steps a lane at every tile length, ragged: by how many workgroups the sizes make."""
+    g = torch.Generator().manual_seed(T)
+    _rec_check(_rec_case(T, B, C, DT[name], lengths=torch.randint(0, T + 1, (B,), generator=g).int()), direction, name)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("T,B,C,gate,h0", [(300, 2, 5, True, True), (33, 1, 1, False, False), (513, 2, 8, False, True), (20, 2, 12, True, False)])
 def test_recurrence_optional_inputs_and_odd_channels(T, B, C, gate, h0, name):
     _rec_check(_rec_case(T, B, C, DT[name], gate, h0), "reverse" if C == 5 else "forward", name)
