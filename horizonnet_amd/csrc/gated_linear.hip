@@ -395,11 +395,17 @@ GlPlan gl_plan(const GlIn& in, bool backward)
         const double longest = (double)(cx > cw ? cx : cw), mean = (double)work / 256;
         p.pp_prod = pp && ldg == ldu && M >= 128 && F >= 64 && 2.0 * (longest > mean ? longest : mean) < 8.0 * M * K * F / 600e6;
         p.prod = gl_product_shape(in.size, M, K, F);
+        long all = 0, tiles[3];
         for (int q = 0; q < 3; ++q) {
-            // few tiles with a long k axis: runs of at least 4 chunks, as many as bring the product to 256 workgroups
-            const long tiles = gl_tiles(I[q], K, gl_shape_i(p.prod), gl_shape_j(p.prod));
-            long s = tiles > 0 ? 256 / tiles : 1;
-            if (s > chunks[q] / 4) s = chunks[q] / 4;
+            tiles[q] = gl_tiles(I[q], K, gl_shape_i(p.prod), gl_shape_j(p.prod));
+            all += tiles[q] * chunks[q];
+        }
+        // a product whose k axis is longer than its share is cut into runs of about the same number of chunks for all: a 256th of the chunks, in
+        // float32, where two workgroups on a unit hide each other's waits, a 512th, and 4 at least (products of M 512, K 512, F 1024 with the rest of the
+        // backward pass: float32 34.3 us by 512, 40.8 by 256; bf16 22.0 by 256, 31.3 by 256 workgroups for each product by itself)
+        const long units = in.size == 2 ? 256 : 512, even = all / units > 4 ? all / units : 4;
+        for (int q = 0; q < 3; ++q) {
+            long s = (2 * chunks[q] + even) / (2 * even);
             if (s < 1 || p.pp_prod) s = 1;
             p.run[q] = (int)((chunks[q] + s - 1) / s);
             if (p.run[q] < 1) p.run[q] = 1;
