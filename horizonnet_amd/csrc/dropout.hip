@@ -2,8 +2,9 @@
 // (seed, i) reach p 2^32.  The generator is the training step's own (seq_dropout_bits in seq_common.h), so dropout(x, p, 2 seed + 1 + l) draws
 // the mask the engine draws behind LSTM layer l.  The gradient of x is the same pass over dy, that of r is dy itself.
 //
-// Bound by HBM: 2 tensors (3 with a residual) against two 64-bit products per element.  16.8 M elements in bf16: 18.5 us with a residual
-// (101 MB, 5.4 TB/s), 15.5 us without (67 MB, 4.3 TB/s); a large copy reaches 5.0.  The seed may lie on the device, where a captured
+// 2 tensors (3 with a residual) against 22 vector instructions an element, six of them the 32-bit products of the generator's two 64-bit ones, which
+// take four times as long as others.  16.8 M elements in bf16: 17.4 us with a residual (101 MB, 5.8 TB/s: HBM), 15.0 us without (67 MB, 4.5 TB/s:
+// the generator, about as long as the traffic); a large copy reaches 5.0.  The seed may lie on the device, where a captured
 // step that adds to it draws a new mask on every replay.
 #include "seq_common.h"
 
