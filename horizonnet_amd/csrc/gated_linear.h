@@ -45,8 +45,9 @@ int hn_launch_gated_linear_pp_products(GlJobs& jobs, hipStream_t s);
 
 namespace {
 
-// Value and slope of the activation.  bf16 (not EXACT): the sigmoid from one exponential and one reciprocal, 1 - s by subtraction: what that
-// loses is far below the step of a bf16 result, which s and 1 - s enter beside terms of their own size.
+// Value and slope of the activation.  bf16 (not EXACT): the sigmoid from one exponential and one reciprocal.  silu takes 1 - s by subtraction, whose
+// loss is far below the step of a bf16 result: s and 1 - s enter its slope beside terms of their own size.  sigmoid's slope s (1 - s) has 1 - s as a bare
+// factor (the subtraction is 17 % off at z 15 and 0 from 17 on), so it is e^-z s there.
 template <bool EXACT>
 __device__ __forceinline__ void gl_act(float z, int act, float& a, float& slope)
 {
@@ -62,8 +63,9 @@ __device__ __forceinline__ void gl_act(float z, int act, float& a, float& slope)
         if constexpr (EXACT) {
             seq_logistic<true>(z, s, rest);
         } else {
-            s = seq_sigmoid<false>(z);
-            rest = 1.f - s;
+            const float e = __expf(-z);
+            s = __builtin_amdgcn_rcpf(1.f + e);
+            rest = act == GL_SIGMOID ? fminf(e, 3.0e38f) * s : 1.f - s;     // (s is 0 where e is infinite)
         }
         if (act == GL_SIGMOID) { a = s; slope = s * rest; }
         else { a = z * s; slope = fmaf(a, rest, s); }
