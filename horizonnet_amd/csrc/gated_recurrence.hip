@@ -415,7 +415,7 @@ __global__ __launch_bounds__(TILE / L * CL, 2) void gated_recurrence_bwd_kernel(
                     seq_logistic<EXACT>(x[k], a, rest);
                     as[i][k] = on ? a : 1.f;
                     rs[i][k] = on ? rest : 0.f;
-                    gs[i][k] = gate ? g[k] * seq_sigmoid<EXACT>(q[k]) : g[k];         // (0 where the step is not taken: g is)
+                    gs[i][k] = gate ? g[k] * seq_sigmoid_full<EXACT>(q[k]) : g[k];    // (0 where the step is not taken: g is)
                     A[k] *= as[i][k];
                     if (PASS == 0) H[k] = fmaf(as[i][k], H[k], rs[i][k] * z[k]);
                 }

@@ -62,24 +62,46 @@ __device__ __forceinline__ void seq_store(T* p, const float (&x)[VEC])
     seq_put(p, x);
 }
 
+// e^x for a factor of a float32 result.  EXACT: x is any float32, the library's exponential.  Else x is a bf16 value: its 8 bits times the 16 of
+// SEQ_LOG2E are exact in float32, so 2^t takes no error from its argument, and what the constant leaves out, x SEQ_LOG2E_REST natural units
+// (at most 5e-4 where the result is a normal number), is a factor 1 + c.  The constant of c is turned by 0.9e-4 to the side of e^c - 1 = c + c^2 / 2 for results
+// below 1 (DOWN) or above.  Off by 4 u (u = 2^-24): 2 of v_exp_f32, 1 of the last sum, 0.9 of e^c.  The short exponential (2 instructions, |x| u) takes 3 fewer.
+constexpr float SEQ_LOG2E = 0x1.7154p0f, SEQ_LOG2E_REST = 4.88849518e-6f;
+template <bool EXACT, bool DOWN>
+__device__ __forceinline__ float seq_exp(float x)
+{
+    if constexpr (EXACT) return expf(x);
+    const float c = __builtin_amdgcn_fmed3f(x * (SEQ_LOG2E_REST * (DOWN ? 0.99991f : 1.00009f)), -0x1p-10f, 0x1p-10f);   // (x may be infinite)
+    const float e = __builtin_amdgcn_exp2f(x * SEQ_LOG2E);
+    return fmaf(e, c, e);
+}
+
 // s(x) and 1 - s(x) = s(-x) from ONE exponential of -|x|: neither is formed by a subtraction from 1, so the small one keeps its relative
-// precision (a long memory is a small 1 - a).  EXACT: float32 outputs; otherwise the 2-instruction exponential, whose relative error
-// |x| 2^-23 is far below a bf16 step.
+// precision (a long memory is a small 1 - a).  Both are right to float32's last bits in both modes: the states that they make are float32, whatever the
+// type of the inputs (exponential 4 u, sum and reciprocal 3 u, product u).
 template <bool EXACT>
 __device__ __forceinline__ void seq_logistic(float x, float& s, float& rest)
 {
-    const float e = EXACT ? expf(-fabsf(x)) : __expf(-fabsf(x));
+    const float e = seq_exp<EXACT, true>(-fabsf(x));
     const float big = __builtin_amdgcn_rcpf(1.0f + e);
     const float small = e * big;
     s = x >= 0.f ? big : small;
     rest = x >= 0.f ? small : big;
 }
 
-// s(x) alone: the exponential's overflow gives the right 0
+// s(x) alone, for a factor of a result that is stored in T.  EXACT: T is float32.  Otherwise the 2-instruction exponential, whose relative error
+// |x| 2^-23 is far below a bf16 step.  Its overflow gives the right 0
 template <bool EXACT>
 __device__ __forceinline__ float seq_sigmoid(float x)
 {
     return __builtin_amdgcn_rcpf(1.0f + (EXACT ? expf(-x) : __expf(-x)));
+}
+
+// s(x) for a factor of a float32 result, in both modes
+template <bool EXACT>
+__device__ __forceinline__ float seq_sigmoid_full(float x)
+{
+    return __builtin_amdgcn_rcpf(1.0f + seq_exp<EXACT, false>(-x));
 }
 
 // The counter-based generator of every dropout here: 32 bits for element `index` of the stream base = seed * SEQ_DROPOUT_STRIDE (a 64-bit

@@ -39,3 +39,45 @@ def test_sigmoid_gate_saturated(name, M, K, F):
     for n, t in zip(("dbg", "dwg"), grads):
         off = ((t.double() - want[n]).abs() / want[n]).max()
         assert float(off) <= room[n] * 1.0001, (n, float(off), room[n])
+
+
+def test_float32_results_of_bf16_recurrence():
+    """The states and dh0 of a bf16 call are float32 and have to be right to float32's last bits: with v = 0 they are products of gates alone.  One
+    gate is off by 2 u for the exponential, u for the correction, u + 2 u for 1 + e and its reciprocal, u for the product: 7 u, and u more for the product
+    with the state; a second gate, of the output, adds as much again (the order in which steps are joined adds u a step)."""
+    u = ref.U
+    g = torch.Generator().manual_seed(3)
+    for T, B, C in ((1, 7, 130), (1, 300, 512), (2, 5, 64)):
+        f = (-80 + 72 * torch.rand(T, B, C, generator=g) if T == 1 else -40 + 32 * torch.rand(T, B, C, generator=g)).bfloat16()
+        o = (-80 + 160 * torch.rand(T, B, C, generator=g)).bfloat16()
+        v, h0 = torch.zeros(T, B, C, dtype=torch.bfloat16), 1 + torch.rand(B, C, generator=g)
+        a = torch.sigmoid(f.double()).prod(0)
+        want = a * h0.double()
+        for direction in ("forward", "both"):
+            leaves = [f.to(DEV).requires_grad_(True), v.to(DEV), o.to(DEV), h0.to(DEV).requires_grad_(True)]
+            y, last = hn.gated_recurrence(leaves[0], leaves[1], out_gate=leaves[2], h0=leaves[3], direction=direction)
+            assert float(((last.detach().cpu().double() - want) / want).abs().max()) <= 8 * T * u
+            with torch.no_grad():
+                assert torch.equal(hn.gated_recurrence(leaves[0], leaves[1], h0=leaves[3], direction=direction)[1], last)
+            dlast = 1 + torch.rand(B, C, generator=g)
+            dh0, = torch.autograd.grad(last, [leaves[3]], dlast.to(DEV), retain_graph=True)
+            w = a * dlast.double()
+            assert float(((dh0.cpu().double() - w) / w).abs().max()) <= 8 * T * u
+            if T == 1:
+                dy = (1 + torch.rand(T, B, C, generator=g)).bfloat16()
+                few = o.clamp(min=-5)                                        # (the product of the two gates stays a normal number)
+                y, last = hn.gated_recurrence(leaves[0], leaves[1], out_gate=few.to(DEV), h0=leaves[3], direction=direction)
+                dh0, = torch.autograd.grad(y, [leaves[3]], dy.to(DEV))
+                w = (torch.sigmoid(f.double()) * torch.sigmoid(few.double()) * dy.double())[0]
+                assert float(((dh0.cpu().double() - w) / w).abs().max()) <= 16 * u
+        if T == 1:
+            state = h0.to(DEV)
+            hn.gated_recurrence_step(f[0].to(DEV), v[0].to(DEV), state)
+            assert float(((state.cpu().double() - want) / want).abs().max()) <= 8 * u
+    steps = (-30 + 60 * torch.rand(1, 1, 4096, generator=g)).bfloat16()      # the other side: 1 - a of a nearly closed gate, and gates at infinity
+    one = torch.ones(1, 1, 4096, dtype=torch.bfloat16)
+    want = torch.sigmoid(-steps.double())[0]
+    assert float(((hn.gated_recurrence(steps.to(DEV), one.to(DEV))[1].cpu().double() - want) / want).abs().max()) <= 8 * u
+    ends = torch.tensor([float("inf"), -float("inf"), 3e38, -3e38, 200.0, -200.0, float("nan")]).bfloat16().view(1, 1, -1).to(DEV)
+    for got in (hn.gated_recurrence(ends, torch.full_like(ends, 2.0), h0=torch.full((1, 7), 9.0, device=DEV))[1][0].tolist(),):
+        assert got[:6] == [9.0, 2.0, 9.0, 2.0, 9.0, 2.0] and got[6] != got[6]
