@@ -81,3 +81,48 @@ def test_float32_results_of_bf16_recurrence():
     ends = torch.tensor([float("inf"), -float("inf"), 3e38, -3e38, 200.0, -200.0, float("nan")]).bfloat16().view(1, 1, -1).to(DEV)
     for got in (hn.gated_recurrence(ends, torch.full_like(ends, 2.0), h0=torch.full((1, 7), 9.0, device=DEV))[1][0].tolist(),):
         assert got[:6] == [9.0, 2.0, 9.0, 2.0, 9.0, 2.0] and got[6] != got[6]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("direction", ["forward", "reverse", "both"])
+@pytest.mark.parametrize("T,B,C", [(30, 2, 6), (60, 3, 40), (120, 2, 64), (120, 40, 520), (300, 2, 36), (1500, 1, 64), (1500, 9, 330)])
+def test_infinite_state_stays(T, B, C, direction, name):
+    """An infinite value makes the state infinite from its step on: a gate above 0 passes it on however many steps follow, also where the product of
+    their gates is no float32 number any more.  The gradient of a state flows back the same way."""
+    g = torch.Generator().manual_seed(T + B)
+    f = (torch.randn(T, B, C, generator=g) * 1.5 - 3).to(DT[name])           # (gates of about 1/20: 30 of them are 1e-39)
+    f[:, :, 1] = -30                                                         # (and in one channel 2 of them)
+    v, h0 = torch.randn(T, B, C, generator=g).to(DT[name]), torch.randn(B, C, generator=g)
+    at, sign = T // 3, torch.where(torch.rand(C, generator=g) < 0.5, -1.0, 1.0)
+    hit = torch.arange(C) % 4 == 1
+    v[at, :, hit] = (float("inf") * sign[hit]).to(DT[name])
+    back = torch.zeros(C, dtype=torch.bool)                                  # channels that run from the last step
+    back[C // 2 if direction == "both" else 0 if direction == "reverse" else C:] = True
+    step = torch.arange(T)[:, None]
+    gone = torch.where(back, step <= at, step >= at) & hit                   # [T, C]: steps whose state is infinite
+    fd, vd, hd = (t.to(DEV).requires_grad_(True) for t in (f, v, h0))
+    y, last = hn.gated_recurrence(fd, vd, h0=hd, direction=direction)
+    got = y.detach().cpu().float()
+    assert bool((got[gone[:, None].expand(T, B, C)] == (sign * float("inf")).expand(T, B, C)[gone[:, None].expand(T, B, C)]).all())
+    assert bool(torch.isfinite(got[~gone[:, None].expand(T, B, C)]).all())
+    assert bool((last.detach().cpu()[:, hit] == (sign * float("inf"))[hit]).all()) and bool(torch.isfinite(last[:, ~hit.to(DEV)]).all())
+    # the gradient of an infinite dy at step `at` is infinite at every step in front of it, and at h0
+    v, dy = torch.randn(T, B, C, generator=g).to(DT[name]), torch.randn(T, B, C, generator=g).to(DT[name])
+    dy[at, :, hit] = (float("inf") * sign[hit]).to(DT[name])
+    gone = torch.where(back, step >= at, step <= at) & hit
+    vd = v.to(DEV).requires_grad_(True)
+    y, last = hn.gated_recurrence(fd, vd, h0=hd, direction=direction)
+    dv, dh0 = torch.autograd.grad(y, [vd, hd], dy.to(DEV))
+    got, full = dv.cpu().float(), gone[:, None].expand(T, B, C)
+    assert bool((got[full] == (sign * float("inf")).expand(T, B, C)[full]).all()) and bool(torch.isfinite(got[~full]).all())
+    assert bool((dh0.cpu()[:, hit] == (sign * float("inf"))[hit]).all()) and bool(torch.isfinite(dh0[:, ~hit.to(DEV)]).all())
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_closed_gate_forgets_exactly(name):
+    """A gate that is 0 leaves nothing of a finite state, on whichever side of a join it lies."""
+    T, C = 1500, 64
+    f, v = torch.full((T, 1, C), 2.0, dtype=DT[name], device=DEV), torch.zeros(T, 1, C, dtype=DT[name], device=DEV)
+    f[700] = -float("inf")
+    y, last = hn.gated_recurrence(f, v, h0=torch.full((1, C), 1e30, device=DEV))
+    assert bool((y[700:] == 0).all()) and bool((last == 0).all()) and bool((y[0] > 1e29).all())
