@@ -70,10 +70,15 @@ __global__ __launch_bounds__(256, 2) void gl_gate_kernel(GlArgs p)
                 for (int e = 0; e < 8; ++e) {
                     float a, slope;
                     gl_act<sizeof(T) == 4>(g[e], p.act, a, slope);
-                    g[e] = d[e] * u[e] * slope;                       // (0 in the columns up to Fp, which the products read: d is)
+                    g[e] = d[e] * u[e] * slope;
                     u[e] = d[e] * a;
                     sg[e] += g[e];
                     su[e] += u[e];
+                }
+                if (left < 8) {                               // the products read the columns up to Fp: 0, also where a row of x is infinite
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e >= left) g[e] = u[e] = 0.f;
                 }
                 gl_store8((T*)p.dgu + m * 2 * p.Fp + f, g, true, 8);
                 gl_store8((T*)p.dgu + m * 2 * p.Fp + p.Fp + f, u, true, 8);

@@ -391,8 +391,13 @@ struct GpGate {
                     for (int e = 0; e < 8; ++e) {
                         float a, slope;
                         gl_act<false>(gv[e], ACT, a, slope);
-                        gv[e] = d[e] * uv[e] * slope;         // (0 in the columns up to Fp, which the products read: d is)
+                        gv[e] = d[e] * uv[e] * slope;
                         uv[e] = d[e] * a;
+                    }
+                    if (left < 8) {                           // the products read the columns up to Fp: 0, also where a row of x is infinite
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (e >= left) gv[e] = uv[e] = 0.f;
                     }
                     if (p.slab) {
 #pragma unroll

@@ -126,3 +126,23 @@ def test_closed_gate_forgets_exactly(name):
     f[700] = -float("inf")
     y, last = hn.gated_recurrence(f, v, h0=torch.full((1, C), 1e30, device=DEV))
     assert bool((y[700:] == 0).all()) and bool((last == 0).all()) and bool((y[0] > 1e29).all())
+
+
+@pytest.mark.parametrize("name,M,K,F", [("f32", 40, 24, 9), ("f32", 40, 136, 9), ("bf16", 40, 24, 9), ("bf16", 300, 64, 203), ("bf16", 8192, 128, 767)])
+def test_infinite_row_with_odd_hidden_units(name, M, K, F):
+    """x of one row infinite, weights positive, relu: dx of that row is +inf as the formula says and not NaN, also where the rows of dg | du are padded
+    to whole vectors; the other rows are what they are without it."""
+    g = torch.Generator().manual_seed(F)
+    dt = DT[name]
+    x, dy = (torch.rand(M, K, generator=g) + 0.5).to(dt), (torch.rand(M, F, generator=g) + 0.5).to(dt)
+    wg, wu = ((torch.rand(F, K, generator=g) + 0.5) / K for _ in range(2))
+    x[7, 3] = float("inf")
+    xd = x.to(DEV).requires_grad_(True)
+    wgd, wud = wg.to(dt).to(DEV), wu.to(dt).to(DEV)
+    y = hn.gated_linear(xd, wgd, wud, activation="relu")
+    dx, = torch.autograd.grad(y, [xd], dy.to(DEV))
+    assert bool(torch.isposinf(y[7]).all()) and bool(torch.isposinf(dx[7]).all())
+    tame = torch.where(torch.isinf(x), torch.ones((), dtype=dt), x).to(DEV).requires_grad_(True)
+    want, = torch.autograd.grad(hn.gated_linear(tame, wgd, wud, activation="relu"), [tame], dy.to(DEV))
+    rest = torch.arange(M) != 7
+    assert torch.equal(dx[rest], want[rest])
