@@ -5,10 +5,13 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include "../../include/horizonnet_hip.h"
 
@@ -37,6 +40,19 @@ T* addr(const Tensor& t)
     return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 1 : 0; }
+
+// What sees torch's own operations alone has to be told: a tangent would be dropped, which counts as zero, and a trace would keep the outputs' memory
+// without what fills it
+void check_seen(const char* who, std::initializer_list<const Tensor*> ts)
+{
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), who,
+                " cannot be traced: a trace does not record its kernels");
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : ts)
+        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), who, " has no forward-mode derivative");
+}
+template <class Optional>
+const Tensor* in(const Optional& t) { return t ? &*t : nullptr; }
 
 void check_main(const char* who, const char* name, const Tensor& t)
 {
@@ -137,6 +153,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         const Tensor &f = saved[0], &v = saved[1], &o = saved[2], &lengths = saved[3], &states = saved[4];
         const int64_t direction = ctx->saved_data["direction"].toInt();
         const c10::DeviceGuard guard(f.device());
+        check_seen("gated_recurrence", {&grads[0], &grads[1]});
         check_capture("gated_recurrence", f);
         const int64_t T = f.size(0), B = f.size(1), C = f.size(2);
         variable_list out(6);
@@ -165,6 +182,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& forget, const Tensor& 
                                             const Maybe& lengths_, const std::string& direction)
 {
     const char* who = "gated_recurrence";
+    check_seen(who, {&forget, &value, in(out_gate), in(h0_)});
     check_main(who, "forget", forget);
     TORCH_CHECK_VALUE(forget.dim() == 3, who, ": forget must be [T, B, C], got shape ", forget.sizes());
     const int64_t dir = direction == "forward" ? 0 : direction == "reverse" ? 1 : direction == "both" ? 2 : -1;
@@ -195,6 +213,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& forget, const Tensor& 
 Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Tensor& state, const Maybe& out_gate)
 {
     const char* who = "gated_recurrence_step";
+    check_seen(who, {&forget, &value, &state, in(out_gate)});
     check_main(who, "forget", forget);
     TORCH_CHECK_VALUE(forget.dim() == 2, who, ": forget must be [B, C], got shape ", forget.sizes());
     const auto dev = forget.device();
@@ -247,6 +266,7 @@ struct Linear : torch::autograd::Function<Linear> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4], &kept = saved[5];
         const c10::DeviceGuard guard(x.device());
+        check_seen("gated_linear", {&grads[0]});
         check_capture("gated_linear", x);
         const int64_t M = x.size(0), K = x.size(1), F = wg.size(0);
         variable_list out(6);
@@ -275,6 +295,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
                     const std::string& activation)
 {
     const char* who = "gated_linear";
+    check_seen(who, {&x, &w_gate, &w_up, in(b_gate), in(b_up)});
     check_main(who, "x", x);
     TORCH_CHECK_VALUE(x.dim() >= 1, who, ": x must be [..., K]");
     const int64_t act = activation == "silu" ? 0 : activation == "gelu" ? 1 : activation == "sigmoid" ? 2 : activation == "relu" ? 3 : -1;
@@ -322,6 +343,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     {
         variable_list out(5);
         Tensor seed;
+        check_seen("dropout", {&grads[0]});
         check_capture("dropout", grads[0]);
         if (ctx->saved_data["tensor"].toBool()) seed = ctx->get_saved_variables()[0];
         {
@@ -337,6 +359,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor dropout(const Tensor& x_, double p, const py::object& seed_, const Maybe& residual_)
 {
     const char* who = "dropout";
+    check_seen(who, {&x_, in(residual_)});
     check_main(who, "x", x_);
     TORCH_CHECK_VALUE(p >= 0.0 && (float)p < 1.0f, who, ": p must be in [0, 1), got ", p);
     Tensor seed, residual;

@@ -7,7 +7,8 @@ engine itself runs (reference ``model.py:222-227,263-266``: bi-LSTM, dropout, li
 
 All take ROCm tensors in float32 or bfloat16 (one type per call; float32 states), run on the current stream, are differentiable
 (once) and give the same bits every time.  There is no CPU fallback.  Argument checks and autograd nodes are native
-(``csrc/sequence_torch.cpp``): a small call is bound by its host time.
+(``csrc/sequence_torch.cpp``): a small call is bound by its host time.  Forward-mode derivatives and tracing (``torch.jit.trace``, ``make_fx``) are
+refused: both would lose what the kernels do.
 
 Calls may be captured into graphs, the first ones too.  A captured backward pass is refused while an eager graph made on the default stream
 still holds one of the operator's leaf inputs: drop that graph first.

@@ -146,3 +146,69 @@ def test_infinite_row_with_odd_hidden_units(name, M, K, F):
     want, = torch.autograd.grad(hn.gated_linear(tame, wgd, wud, activation="relu"), [tame], dy.to(DEV))
     rest = torch.arange(M) != 7
     assert torch.equal(dx[rest], want[rest])
+
+
+def _calls(x):
+    """The four operators on x [4, 2, 8]."""
+    w = torch.ones(3, 8, device=DEV)
+    other = torch.zeros(4, 2, 8, device=DEV)
+    return [lambda: hn.gated_recurrence(x, other), lambda: hn.gated_recurrence(other, x), lambda: hn.gated_recurrence(other, other, out_gate=x),
+            lambda: hn.gated_recurrence(other, other, h0=x[0]), lambda: hn.gated_linear(x, w, w), lambda: hn.gated_linear(other, x[:, 0, :], w[:1].expand(4, 8)),
+            lambda: hn.dropout(x, 0.5, 1), lambda: hn.dropout(other, 0.5, 1, residual=x),
+            lambda: hn.gated_recurrence_step(x[0], other[0], torch.zeros(2, 8, device=DEV)),
+            lambda: hn.gated_recurrence_step(other[0], other[0], torch.zeros(2, 8, device=DEV), out_gate=x[0])]
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be dropped: refused, with and without requires_grad, with and without grad mode."""
+    with torch.autograd.forward_ad.dual_level():
+        for primal in (torch.randn(4, 2, 8, device=DEV), torch.randn(4, 2, 8, device=DEV, requires_grad=True)):
+            dual = torch.autograd.forward_ad.make_dual(primal, torch.ones(4, 2, 8, device=DEV))
+            for call in _calls(dual):
+                with pytest.raises(RuntimeError):
+                    call()
+                with torch.no_grad(), pytest.raises(RuntimeError):
+                    call()
+    x = torch.randn(4, 2, 8, device=DEV)
+    for transform in (lambda fn: torch.func.jvp(fn, (x,), (x,)), lambda fn: torch.func.vmap(fn)(x[None]), lambda fn: torch.func.grad(lambda t: fn(t).sum())(x)):
+        with pytest.raises(RuntimeError):
+            transform(lambda t: hn.dropout(t, 0.5, 1))
+        with pytest.raises(RuntimeError):
+            transform(lambda t: hn.gated_recurrence(t, t)[0])
+
+
+def test_tracing_is_refused():
+    """A trace sees the outputs' memory and nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(4, 2, 8, device=DEV)
+    for k in range(len(_calls(x))):
+        def fn(t):
+            y = _calls(t)[k]()
+            return y[0] if isinstance(y, tuple) else y
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                torch.jit.trace(fn, (x,), check_trace=False)
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                make_fx(fn)(x)
+
+
+def test_backward_is_seen_too():
+    """The same in a backward pass whose forward pass ran outside: an incoming gradient with a tangent, a trace of the backward pass alone."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, w = torch.randn(4, 2, 8, device=DEV, requires_grad=True), torch.randn(8, 8, device=DEV)
+    dy = torch.randn(4, 2, 8, device=DEV)
+    for call in (lambda: hn.gated_recurrence(x, x)[0], lambda: hn.gated_linear(x, w, w), lambda: hn.dropout(x, 0.5, 1)):
+        y = call()
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(y, x, torch.autograd.forward_ad.make_dual(dy, dy), retain_graph=True)
+        for trace in (lambda fn: torch.jit.trace(fn, (dy,), check_trace=False), lambda fn: make_fx(fn)(dy)):
+            with pytest.raises(RuntimeError):
+                trace(lambda d: torch.autograd.grad(y, x, d, retain_graph=True)[0])
+        assert torch.autograd.grad(y, x, dy)[0].shape == x.shape
+    last = hn.gated_recurrence(x, x)[1]
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.autograd.grad(last, x, torch.autograd.forward_ad.make_dual(dy[0], dy[0]))
