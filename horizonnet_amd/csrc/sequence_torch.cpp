@@ -13,6 +13,9 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
+#include <unordered_set>
+#include <vector>
+
 #include "../../include/horizonnet_hip.h"
 
 namespace {
@@ -96,7 +99,28 @@ variable_list once(const char* who, variable_list grads)
 }
 
 // A gradient accumulator that an eager graph keeps alive belongs to the stream that graph was made on.  On its way there a captured backward
-// pass would draw the default stream into the capture, which ends the process: refused before that.
+// pass would draw the default stream into the capture, which ends the process: refused before that.  The operator's own leaves count, and every node
+// that this pass will run behind it (the leaf may lie behind a reshaped batch, the copy of an input whose channels lie apart, a cast weight)
+bool draws_default_stream(torch::autograd::Node* node)
+{
+    std::vector<torch::autograd::Node*> todo{node};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!todo.empty()) {
+        const auto at = todo.back();
+        todo.pop_back();
+        for (size_t i = 0; i < at->num_outputs(); ++i) {
+            const auto next = at->next_edge(i).function.get();
+            if (!next) continue;
+            const bool run = at->task_should_compute_output(i);
+            if (run || (at == node && dynamic_cast<torch::autograd::AccumulateGrad*>(next))) {
+                const auto its = next->stream();
+                if (its && its->id() == 0) return true;
+            }
+            if (run && seen.insert(next).second) todo.push_back(next);
+        }
+    }
+    return false;
+}
 void check_capture(const char* who, const Tensor& t)
 {
     const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device());
@@ -104,12 +128,8 @@ void check_capture(const char* who, const Tensor& t)
     if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
-    for (const auto& edge : node->next_edges()) {
-        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
-        const auto its = edge.function->stream();
-        TORCH_CHECK(!its || its->id() != 0, who, ": the backward pass is being captured while a graph made on the default stream holds one of its leaves; "
-                    "let go of that graph first, or make it on a side stream");
-    }
+    TORCH_CHECK(!draws_default_stream(node.get()), who, ": the backward pass is being captured while a graph made on the default stream holds one of its leaves; "
+                "let go of that graph first, or make it on a side stream");
 }
 
 // ---- gated linear recurrence ----

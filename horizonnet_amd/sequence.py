@@ -11,7 +11,7 @@ All take ROCm tensors in float32 or bfloat16 (one type per call; float32 states)
 refused: both would lose what the kernels do.
 
 Calls may be captured into graphs, the first ones too.  A captured backward pass is refused while an eager graph made on the default stream
-still holds one of the operator's leaf inputs: drop that graph first.
+still holds one of the operator's leaf inputs, or a leaf that the pass reaches behind it: drop that graph first.
 """
 _native = None
 

@@ -212,3 +212,48 @@ def test_backward_is_seen_too():
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="no forward-mode derivative"):
             torch.autograd.grad(last, x, torch.autograd.forward_ad.make_dual(dy[0], dy[0]))
+
+
+def _behind(kind):
+    """A leaf on the device and the operator's output through a node of torch between them."""
+    other, weight = torch.randn(4, 2, 64, device=DEV), torch.randn(32, 64, device=DEV)
+    if kind == "batch":                                       # x is reshaped to a matrix
+        leaf = torch.randn(4, 2, 64, device=DEV, requires_grad=True)
+        return leaf, lambda: hn.gated_linear(leaf, weight, weight)
+    if kind == "weight":                                      # rows of a transposed weight are copied
+        leaf = torch.randn(64, 32, device=DEV, requires_grad=True)
+        return leaf, lambda: hn.gated_linear(other, leaf.t(), weight)
+    if kind == "cast":
+        leaf = torch.randn(32, 64, device=DEV, requires_grad=True)
+        return leaf, lambda: hn.gated_linear(other.bfloat16(), leaf.bfloat16(), weight.bfloat16())
+    leaf = torch.randn(64, 4, 2, device=DEV).permute(1, 2, 0).requires_grad_(True)      # channels apart
+    assert leaf.is_leaf and leaf.stride(-1) != 1
+    return leaf, {"forget": lambda: hn.gated_recurrence(leaf, other)[0], "value": lambda: hn.gated_recurrence(other, leaf)[0],
+                  "out_gate": lambda: hn.gated_recurrence(other, other, out_gate=leaf)[0], "h0": lambda: hn.gated_recurrence(other, other, h0=leaf[0])[0],
+                  "x": lambda: hn.gated_linear(leaf, weight, weight), "dropout": lambda: hn.dropout(leaf, 0.5, 1),
+                  "residual": lambda: hn.dropout(other, 0.5, 1, residual=leaf)}[kind]
+
+
+@pytest.mark.parametrize("kind", ["batch", "weight", "cast", "forget", "value", "out_gate", "h0", "x", "dropout", "residual"])
+def test_captured_backward_of_leaves_behind_a_view(kind):
+    """A leaf that an eager graph on the default stream holds is refused also where a node of torch stands between it and the operator; once that graph is
+    gone the capture works."""
+    leaf, call = _behind(kind)
+    held = call()
+    dy = torch.randn_like(held)
+    want = torch.autograd.grad(held, leaf, dy, retain_graph=True)[0]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="being captured while a graph"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(call(), leaf, dy)
+    torch.cuda.synchronize()
+    assert torch.equal(torch.autograd.grad(held, leaf, dy)[0], want)
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call(), leaf, dy)[0]
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
