@@ -230,6 +230,18 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& forget, const Tensor& 
     return {r.y, r.last};
 }
 
+// Whether t [B, C] shares memory with the contiguous state, other than by being it: a thread reads its own elements alone before it writes them, so
+// the same tensor may be both, but not one shifted against the other
+bool meets(const Tensor& state, const Tensor& t)
+{
+    if (!t.defined() || t.numel() == 0) return false;
+    const auto s0 = (intptr_t)state.data_ptr(), s1 = s0 + (intptr_t)state.nbytes(), t0 = (intptr_t)t.data_ptr();
+    const int64_t size = (int64_t)t.element_size(), B = t.size(0), width = t.size(1) * size, step = t.stride(0) * size;
+    if (t0 == s0 && t.scalar_type() == state.scalar_type() && (B == 1 || step == width)) return false;
+    const int64_t first = t0 + width > s0 || step == 0 ? 0 : (s0 - t0 - width) / step + 1;         // the first row that ends behind the state's start
+    return first < B && t0 + first * step + width > s0 && t0 + first * step < s1;
+}
+
 Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Tensor& state, const Maybe& out_gate)
 {
     const char* who = "gated_recurrence_step";
@@ -245,6 +257,7 @@ Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Te
     TORCH_CHECK(!wants_grad({&forget, &value, &o, &state}), who, " is not differentiable: call it under torch.no_grad() or use gated_recurrence");
     const at::AutoGradMode off(false);
     const Tensor f = rows(forget), v = rows(value);
+    TORCH_CHECK(!meets(state, f) && !meets(state, v) && !meets(state, o), who, ": state is updated in place and shares memory with an input");
     const c10::DeviceGuard guard(dev);
     Tensor y = at::empty(forget.sizes(), f.options());
     check(hn_gated_recurrence_step(addr(f), f.stride(0), addr(v), v.stride(0), addr(o), stride_of(o, 0), addr<float>(state), addr(y), f.size(0), f.size(1),

@@ -44,7 +44,8 @@ def gated_recurrence(forget, value, out_gate=None, h0=None, lengths=None, direct
 
 def gated_recurrence_step(forget, value, state, out_gate=None):
     """One step of ``gated_recurrence`` for a serving loop: forget, value, out_gate ``[B, C]``; state float32 ``[B, C]``, contiguous, is updated
-    IN PLACE; returns y ``[B, C]``.  Not differentiable: refuses inputs that ask for gradients."""
+    IN PLACE and overlaps no input in part (an input may be the state itself); returns y ``[B, C]``.  Not differentiable: refuses inputs that ask
+    for gradients."""
     return (_native or _load()).gated_recurrence_step(forget, value, state, out_gate)
 
 

@@ -257,3 +257,31 @@ def test_captured_backward_of_leaves_behind_a_view(kind):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_step_refuses_a_state_that_overlaps_an_input():
+    """The state is written while other elements' inputs are read: an input that lies over it in part is refused; one that is the state itself, or lies beside
+    or between its rows, is taken."""
+    buf = torch.randn(64, device=DEV)
+    state = buf[16:32].view(2, 8)
+    far = torch.randn(2, 8, device=DEV)
+    over = [buf[8:24].view(2, 8), buf[24:40].view(2, 8), buf[17:33].view(2, 8), buf.as_strided((2, 8), (24, 1), 0), buf.as_strided((2, 8), (20, 1), 4),
+            buf.as_strided((2, 8), (0, 1), 20), buf.as_strided((2, 8), (16, 1), 16), buf.as_strided((2, 8), (31, 1), 0)]
+    before = buf.clone()
+    for t in over:
+        for call in (lambda: hn.gated_recurrence_step(t, far, state), lambda: hn.gated_recurrence_step(far, t, state),
+                     lambda: hn.gated_recurrence_step(far, far, state, out_gate=t)):
+            with pytest.raises(RuntimeError, match="shares memory"):
+                call()
+    half = torch.randn(2, 8, device=DEV).bfloat16()
+    with pytest.raises(RuntimeError, match="shares memory"):
+        hn.gated_recurrence_step(buf.view(torch.bfloat16)[32:48].view(2, 8), half, state)
+    assert torch.equal(buf, before)
+    beside = [buf[:16].view(2, 8), buf[32:48].view(2, 8), buf.as_strided((2, 8), (24, 1), 8), buf.as_strided((2, 8), (0, 1), 8), state]
+    for t in beside + [state[:, [3, 1, 2, 0, 5, 6, 7, 4]], buf.as_strided((2, 8), (8, 2), 12)]:            # (copies: channels apart)
+        want = state.clone()
+        y = hn.gated_recurrence_step(t.clone(), far, want)
+        with torch.no_grad():
+            keep = state.clone()
+            assert torch.equal(hn.gated_recurrence_step(t, far, state), y) and torch.equal(state, want)
+            state.copy_(keep)
