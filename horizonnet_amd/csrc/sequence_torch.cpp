@@ -69,9 +69,16 @@ void check_like(const char* who, const char* name, const Tensor& t, at::IntArray
     TORCH_CHECK_VALUE(t.scalar_type() == dtype, who, ": ", name, " is ", t.scalar_type(), ", expected ", dtype);
     TORCH_CHECK_VALUE(t.sizes() == shape, who, ": ", name, " has shape ", t.sizes(), ", expected ", shape);
 }
+// What a kernel reads: a view whose sign is pending (torch's imaginary part of a conjugate is one, and so is the gradient that reaches an imaginary part) is
+// copied with its sign
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // channels next to each other; the other axes as they are
-Tensor rows(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-Tensor whole(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor rows(const Tensor& t_)
+{
+    const Tensor t = plain(t_);
+    return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+Tensor whole(const Tensor& t) { return t.defined() ? plain(t).contiguous() : t; }
 // row stride of a matrix; of a single row any: the one that keeps it aligned
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 int64_t stride_of(const Tensor& t, int axis) { return t.defined() ? t.stride(axis) : 0; }
@@ -213,13 +220,13 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& forget, const Tensor& 
     check_like(who, "value", value, forget.sizes(), dt, dev);
     Tensor o, h0, lengths;
     if (out_gate) { check_like(who, "out_gate", *out_gate, forget.sizes(), dt, dev); o = rows(*out_gate); }
-    if (h0_) { check_like(who, "h0", *h0_, {B, C}, at::kFloat, dev); h0 = h0_->contiguous(); }
+    if (h0_) { check_like(who, "h0", *h0_, {B, C}, at::kFloat, dev); h0 = whole(*h0_); }
     TORCH_CHECK_VALUE(dir != 2 || C % 2 == 0, who, ": direction 'both' needs an even number of channels, got ", C);
     if (lengths_) {
         const auto lt = lengths_->scalar_type();
         TORCH_CHECK_TYPE(lt == at::kInt || lt == at::kLong, who, ": lengths must be an int32 or int64 tensor");
         check_like(who, "lengths", *lengths_, {B}, lt, dev);
-        lengths = lt == at::kInt ? lengths_->contiguous() : lengths_->clamp(0, T).to(at::kInt);
+        lengths = lt == at::kInt ? whole(*lengths_) : lengths_->clamp(0, T).to(at::kInt);
     }
     const Tensor f = rows(forget), v = rows(value);
     if (wants_grad({&f, &v, &o, &h0})) {
@@ -253,7 +260,7 @@ Tensor gated_recurrence_step(const Tensor& forget, const Tensor& value, const Te
     Tensor o;
     if (out_gate) { check_like(who, "out_gate", *out_gate, forget.sizes(), forget.scalar_type(), dev); o = rows(*out_gate); }
     check_like(who, "state", state, forget.sizes(), at::kFloat, dev);
-    TORCH_CHECK_VALUE(state.is_contiguous(), who, ": state is updated in place and must be contiguous");
+    TORCH_CHECK_VALUE(state.is_contiguous() && !state.is_neg(), who, ": state is updated in place and must be contiguous");
     TORCH_CHECK(!wants_grad({&forget, &value, &o, &state}), who, " is not differentiable: call it under torch.no_grad() or use gated_recurrence");
     const at::AutoGradMode off(false);
     const Tensor f = rows(forget), v = rows(value);
@@ -340,8 +347,8 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
     check_like(who, "w_gate", w_gate, {F, K}, dt, dev);
     check_like(who, "w_up", w_up, {F, K}, dt, dev);
     Tensor bg, bu;
-    if (b_gate) { check_like(who, "b_gate", *b_gate, {F}, dt, dev); bg = b_gate->contiguous(); }
-    if (b_up) { check_like(who, "b_up", *b_up, {F}, dt, dev); bu = b_up->contiguous(); }
+    if (b_gate) { check_like(who, "b_gate", *b_gate, {F}, dt, dev); bg = whole(*b_gate); }
+    if (b_up) { check_like(who, "b_up", *b_up, {F}, dt, dev); bu = whole(*b_up); }
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
     const Tensor x2 = rows(x.dim() == 2 ? x : x.reshape({M, K})), wg = rows(w_gate), wu = rows(w_up);
@@ -382,7 +389,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         {
             at::AutoGradMode off(false);
             if (ctx->needs_input_grad(0))
-                out[0] = drop(grads[0].contiguous(), Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["number"].toInt(), seed);
+                out[0] = drop(whole(grads[0]), Tensor(), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["number"].toInt(), seed);
             if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) out[1] = grads[0];
         }
         return once("dropout", std::move(out));
@@ -398,7 +405,7 @@ Tensor dropout(const Tensor& x_, double p, const py::object& seed_, const Maybe&
     Tensor seed, residual;
     uint64_t number = 0;
     if (THPVariable_Check(seed_.ptr())) {
-        seed = THPVariable_Unpack(seed_.ptr());
+        seed = plain(THPVariable_Unpack(seed_.ptr()));
         TORCH_CHECK_VALUE(seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x_.device(), who, ": a seed tensor must be one int64 on ",
                           x_.device(), ", got ", seed.sizes(), " ", seed.scalar_type(), " on ", seed.device());
     } else {
@@ -412,9 +419,9 @@ Tensor dropout(const Tensor& x_, double p, const py::object& seed_, const Maybe&
     py::gil_scoped_release free;
     if (residual_) {
         check_like(who, "residual", *residual_, x_.sizes(), x_.scalar_type(), x_.device());
-        residual = residual_->contiguous();
+        residual = whole(*residual_);
     }
-    const Tensor x = x_.contiguous();
+    const Tensor x = whole(x_);
     if (wants_grad({&x, &residual})) return Dropout::apply(x, maybe(residual), p, (int64_t)number, maybe(seed));
     return drop(x, residual, p, number, seed);
 }

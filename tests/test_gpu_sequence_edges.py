@@ -285,3 +285,45 @@ def test_step_refuses_a_state_that_overlaps_an_input():
             keep = state.clone()
             assert torch.equal(hn.gated_recurrence_step(t, far, state), y) and torch.equal(state, want)
             state.copy_(keep)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_negated_views(name):
+    """A view whose sign is pending (torch's imaginary part of a conjugate) is read with its sign."""
+    g = torch.Generator().manual_seed(17)
+    n = lambda *s: torch.randn(*s, generator=g).to(DT[name]).to(DEV)  # noqa: E731
+    neg = torch._neg_view
+    f, v, o, h0, w, b = n(5, 3, 8), n(5, 3, 8), n(5, 3, 8), torch.randn(3, 8, generator=g).to(DEV), n(4, 8), n(4)
+    for a, c in zip(hn.gated_recurrence(neg(f), neg(v), out_gate=neg(o), h0=neg(h0)), hn.gated_recurrence(-f, -v, out_gate=-o, h0=-h0)):
+        assert torch.equal(a, c)
+    assert torch.equal(hn.gated_linear(neg(f), neg(w), neg(w), neg(b), neg(b)), hn.gated_linear(-f, -w, -w, -b, -b))
+    assert torch.equal(hn.dropout(neg(f), 0.5, 3, residual=neg(v)), hn.dropout(-f, 0.5, 3, residual=-v))
+    s1, s2 = h0.clone(), h0.clone()
+    assert torch.equal(hn.gated_recurrence_step(neg(f[0]), neg(v[0]), s1, out_gate=neg(o[0])), hn.gated_recurrence_step(-f[0], -v[0], s2, out_gate=-o[0]))
+    assert torch.equal(s1, s2)
+    with pytest.raises(ValueError):
+        hn.gated_recurrence_step(f[0], v[0], neg(s1))
+    # gradients that arrive negated
+    leaf = [t.detach().clone().requires_grad_(True) for t in (f, v, h0)]
+    y, last = hn.gated_recurrence(leaf[0], leaf[1], h0=leaf[2])
+    dy, dl = n(5, 3, 8), torch.randn(3, 8, generator=g).to(DEV)
+    for a, c in zip(torch.autograd.grad((y, last), leaf, (neg(dy), neg(dl)), retain_graph=True), torch.autograd.grad((y, last), leaf, (-dy, -dl))):
+        assert torch.equal(a, c)
+    x = f.detach().clone().requires_grad_(True)
+    z = hn.gated_linear(x, w, w)
+    d = n(5, 3, 4)
+    assert torch.equal(torch.autograd.grad(z, x, neg(d), retain_graph=True)[0], torch.autograd.grad(z, x, -d)[0])
+    z = hn.dropout(x, 0.5, 1, residual=x)
+    assert torch.equal(torch.autograd.grad(z, x, neg(dy), retain_graph=True)[0], torch.autograd.grad(z, x, -dy)[0])
+
+
+def test_imaginary_part():
+    """One hidden unit as the imaginary part of a number that is conjugated later: its gradient arrives as such a view."""
+    g = torch.Generator().manual_seed(18)
+    x, w = torch.randn(6, 16, generator=g).to(DEV).requires_grad_(True), torch.randn(1, 16, generator=g).to(DEV)
+    factor = torch.randn(6, 1, generator=g).to(DEV)
+    y = hn.gated_linear(x, w, w)
+    got, = torch.autograd.grad((torch.complex(torch.zeros_like(y), y).conj() * torch.complex(torch.zeros_like(factor), factor)).real.sum(), x)
+    y = hn.gated_linear(x, w, w)
+    want, = torch.autograd.grad((y * factor).sum(), x)
+    assert torch.equal(got, want)
