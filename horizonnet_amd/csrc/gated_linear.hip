@@ -467,7 +467,7 @@ template <typename T, int TI, int TJ, bool BWD>
 int gl_gate_run(const GlArgs& p, hipStream_t s)
 {
     const long n = gl_tiles(p.M, p.F, TI, TJ / 2);
-    HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear: too many tiles");
+    SEQ_REQUIRE_GRID(n, 256, "hn_gated_linear");
     static bool told[64] = {};
     if (const int rc = gl_big_lds(reinterpret_cast<const void*>(gl_gate_kernel<T, TI, TJ, BWD>), gl_lds_bytes<TI, TJ>(), told)) return rc;
     hipLaunchKernelGGL((gl_gate_kernel<T, TI, TJ, BWD>), dim3((unsigned)n), dim3(256), (gl_lds_bytes<TI, TJ>()), s, p);
@@ -497,7 +497,7 @@ int gl_products_run(GlJobs& jobs, hipStream_t s)
         j.tiles = gl_tiles(j.I, j.J, TI, TJ);
         j.first = (int)n;
         n += j.tiles * j.splits;
-        HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear_bwd: too many tiles");
+        SEQ_REQUIRE_GRID(n, 256, "hn_gated_linear_bwd");
     }
     if (n == 0) return 0;
     static bool told[64] = {};
@@ -542,7 +542,7 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
     p.slab = dbg || dbu ? (float*)(ws + pl.slab) : nullptr;
     if (in.M > 0 && in.F > 0 && p.kept) {
         const long n = gl_tiles(in.M, in.F, 64, 64);
-        HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_linear_bwd: too many tiles");
+        SEQ_REQUIRE_GRID(n, 256, "hn_gated_linear_bwd");
         hipLaunchKernelGGL(gl_slope_kernel, dim3((unsigned)n), dim3(256), 0, s, p);
         HN_LAUNCH_CHECK();
     } else if (in.M > 0 && in.F > 0)
@@ -587,7 +587,7 @@ int gl_backward(const GlIn& in, GlArgs p, char* ws, void* dx, void* dwg, void* d
         fin.up = dbu;
     }
     if (planes) {
-        HN_REQUIRE((most + 63) / 64 <= 0x7fffffffL, "hn_gated_linear_bwd: too many results");
+        SEQ_REQUIRE_GRID((most + 63) / 64, 256, "hn_gated_linear_bwd");
         hipLaunchKernelGGL((gl_finish_kernel<T>), dim3((unsigned)((most + 63) / 64), planes), dim3(256), 0, s, fin, bias);
     }
     HN_LAUNCH_CHECK();

@@ -560,7 +560,8 @@ int hn_launch_gated_linear_pp_products(GlJobs& jobs, hipStream_t s)
         j.tiles = (long)hn_cdiv(j.I, 256) * j.tj;
         j.first = (int)n;
         n += j.tiles;
-        HN_REQUIRE(n <= 0x3fffffffL && j.splits == 1 && j.chunks >= 1, "hn_gated_linear_bwd: too many tiles");
+        HN_REQUIRE(j.splits == 1 && j.chunks >= 1, "hn_gated_linear_bwd: a product of whole k axes");
+        SEQ_REQUIRE_GRID(n, 512, "hn_gated_linear_bwd");
     }
     if (n == 0) return 0;
     hipLaunchKernelGGL(gl_product_pp_kernel, dim3((unsigned)n), dim3(512), GP_LDS, s, jobs);

@@ -640,7 +640,7 @@ int rec_launch(RecArgs p, const RecPlan& plan, hipStream_t s)
     p.S = plan.S;
     p.span = plan.span;
     const long n = (long)p.groups * p.dirs * p.B * p.S;
-    HN_REQUIRE(n <= 0x7fffffffL, "hn_gated_recurrence: too many sequences x channels");
+    SEQ_REQUIRE_GRID(n, TILE / L * CL, "hn_gated_recurrence");
     const dim3 grid((unsigned)n), block(TILE / L * CL);
     if constexpr (BWD) {
         if constexpr (TILE == SHORT)              // (the other tiles are never cut into spans)
@@ -750,7 +750,7 @@ extern "C" int hn_gated_recurrence_step(const void* f, int64_t f_b, const void* 
     HN_REQUIRE(f && v && state && y, "hn_gated_recurrence_step: null pointer");
     const bool v4 = C % 4 == 0;           // (lanes that shared channels would update the state twice)
     const long n = B * (v4 ? C / 4 : C);
-    HN_REQUIRE((n + 255) / 256 <= 0x7fffffffL, "hn_gated_recurrence_step: too many sequences x channels");
+    SEQ_REQUIRE_GRID((n + 255) / 256, 256, "hn_gated_recurrence_step");
     const dim3 grid((unsigned)((n + 255) / 256));
     hipStream_t s = (hipStream_t)stream;
 #define HN_STEP(T, VEC) \

@@ -2,6 +2,11 @@
 #pragma once
 #include "hn_common.h"
 
+// A launch holds fewer than 2^32 threads, whatever its number of workgroups
+#define SEQ_REQUIRE_GRID(blocks, threads, what)                                                                             \
+    HN_REQUIRE((long)(blocks) * (threads) < (1L << 32), what ": too large: %ld workgroups of %d threads, and a launch holds fewer than 2^32 threads", \
+               (long)(blocks), (int)(threads))
+
 namespace {
 
 typedef unsigned short seq_bf16;      // storage of one bf16 value

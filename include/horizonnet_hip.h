@@ -424,7 +424,8 @@ int hn_linear_head(const float* y, const float* w, const float* bias, float* bon
                    int T, int B, void* stream);
 
 /* ---- sequence operators: the pieces of a recurrent block over the [T][B][C] sequence that hn_upsample_flatten builds and the LSTM layers
- * read.  dtype: 0 float32, 1 bf16 (every tensor below that is `void*`; `float*` ones are float32 always).  Strides count elements. ---- */
+ * read.  dtype: 0 float32, 1 bf16 (every tensor below that is `void*`; `float*` ones are float32 always).  Strides count elements.  A launch holds fewer
+ * than 2^32 threads: sizes that would need more (2^26 sequences of one step and one channel) are refused. ---- */
 
 /* Gated linear recurrence, every channel by itself:  a = s(f), h_t = a_t h_{t-1} + (1 - a_t) v_t, y_t = s(o_t) h_t  (s: logistic function).
  * f, v, o [T][B][C] by their time and sequence strides, channels contiguous; o may be null (y = h).  direction: 0 from the first step,

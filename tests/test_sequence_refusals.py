@@ -1,8 +1,11 @@
 """Calls of the sequence operators that the host has to refuse, without a GPU: each check comes before any launch."""
+import ctypes
+
 import pytest
 import torch
 
 import horizonnet_amd as hn
+from horizonnet_amd import _lib
 
 
 def _calls(x):
@@ -39,3 +42,26 @@ def test_tracing_is_refused():
         for trace in (lambda fn: torch.jit.trace(fn, (x,), check_trace=False), lambda fn: make_fx(fn)(x)):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 trace(lambda t: _calls(t)[k]())
+
+
+def _fails(rc, text):
+    assert rc != 0 and text in _lib.load().hn_last_error().decode()
+
+
+def test_launches_past_2_32_threads_are_refused():
+    """Sizes inside each argument's own range whose launch would hold 2^32 threads or more (a step of 2^32 sequences, rows of one hidden unit, ...)."""
+    lib, one = _lib.load(), ctypes.c_void_p(256)              # an address that is never read
+    for T, B, C, direction in ((1, 1 << 26, 1, 0), (1, 1 << 26, 3, 1), (50, 1 << 25, 1, 0), (100, 1 << 24, 2, 2), (1, (1 << 31) - 1, 1 << 20, 0)):
+        for dtype in (0, 1):
+            n = lib.hn_gated_recurrence_workspace(T, B, C, direction)
+            assert n == 0
+            _fails(lib.hn_gated_recurrence(one, C, C, one, C, C, None, 0, 0, None, None, one, one, None, None, 0, T, B, C, dtype, direction, None), "2^32 threads")
+            _fails(lib.hn_gated_recurrence_bwd(one, C, C, one, C, C, None, 0, 0, one, C, C, None, None, one, one, one, None, None, None, 0, T, B, C, dtype, direction,
+                                               None), "2^32 threads")
+    for B, C in (((1 << 31) - 1, 3), ((1 << 31) - 1, 8), (1 << 20, 1 << 14)):
+        _fails(lib.hn_gated_recurrence_step(one, C, one, C, None, 0, one, one, B, C, 0, None), "2^32 threads")
+    for dtype in (0, 1):
+        _fails(lib.hn_gated_linear(one, 8, one, 8, one, 8, None, None, one, None, None, 0, (1 << 31) - 1, 8, 1, dtype, 0, None), "2^32 threads")
+        need = lib.hn_gated_linear_workspace(one, 8, one, 8, one, 8, (1 << 31) - 1, 8, 1, dtype, 1)
+        _fails(lib.hn_gated_linear_bwd(one, 8, one, 8, one, 8, None, None, one, 1, None, one, one, one, None, None, one, need, (1 << 31) - 1, 8, 1, dtype, 0, None),
+               "2^32 threads")
