@@ -35,11 +35,23 @@ PY
       ;;
   esac
 }
+# an object is rebuilt where its source, a header or this script, which holds its flags, is newer
+HEADERS="*.h ../../include/horizonnet_hip.h"
+stale() {      # source, object
+  local d
+  [ -f "$2" ] || return 0
+  for d in "$1" $HEADERS build.sh; do [ "$d" -nt "$2" ] && return 0; done
+  return 1
+}
+if [ -n "${HN_BUILD_LIST:-}" ]; then      # say what would be compiled, and stop
+  for f in $SRCS; do if stale "$f" "$OBJDIR/${f%.hip}.o"; then echo "$f"; fi; done
+  exit 0
+fi
 PIDS=""
 OBJS=""
 for f in $SRCS; do
   o=$OBJDIR/${f%.hip}.o
-  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ hn_common.h -nt "$o" ] || [ engine_internal.h -nt "$o" ] || [ multi_job.h -nt "$o" ] || [ conv_bf16_args.h -nt "$o" ] || [ conv_bf16_pp.h -nt "$o" ] || [ seq_common.h -nt "$o" ] || [ gated_linear.h -nt "$o" ] || [ gated_linear_tile.h -nt "$o" ] || [ stat_commit.h -nt "$o" ] || [ stat_wave.h -nt "$o" ] || [ ../../include/horizonnet_hip.h -nt "$o" ]; then
+  if stale "$f" "$o"; then
     compile "$f" "$o" &
     PIDS="$PIDS $!"
     if [ $(jobs -rp | wc -l) -ge ${HN_BUILD_JOBS:-8} ]; then wait -n || exit 1; fi
