@@ -385,6 +385,9 @@ struct GpGate {
                     if (rd + RING < 8) ring[rd & (RING - 1)] = *reinterpret_cast<const gl_u32x4*>(pd + 16L * (rd + RING) * p.ldd);
                 } else if (on) {
                     gl_load8((const seq_bf16*)p.dy + m * p.ldd + f, d, p.dy_vec, left);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)               // the products read the columns up to Fp: 0, also where a row of x is infinite
+                        if (e >= left) gv[e] = uv[e] = 0.f;
                 }
                 if (on) {
 #pragma unroll
@@ -393,11 +396,6 @@ struct GpGate {
                         gl_act<false>(gv[e], ACT, a, slope);
                         gv[e] = d[e] * uv[e] * slope;
                         uv[e] = d[e] * a;
-                    }
-                    if (left < 8) {                           // the products read the columns up to Fp: 0, also where a row of x is infinite
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (e >= left) gv[e] = uv[e] = 0.f;
                     }
                     if (p.slab) {
 #pragma unroll
