@@ -13,8 +13,8 @@
 //             launch, a workgroup per tile, longest k first, so that unequal jobs still fill the device.
 //
 // Bound by the matrix pipe and, between a tile's last product and the next one's first, by the epilogue that all compute units reach at about the
-// same time.  M 8192, K 1024, F 4096: gate 140 us forward (0.98 PFLOP/s), 172 us backward (dy read, dg | du written), the products 264 us (1.04
-// PFLOP/s); M 16384 forward 250 us (1.10).  A large library product reaches 1.26 on the same card.
+// same time.  M 8192, K 1024, F 4096: gate 140 us forward (0.98 PFLOP/s), 177 us backward (dy read, dg | du written), the products 257 - 280 us (1.07 -
+// 0.98 PFLOP/s, by card); M 16384 forward 248 us (1.11).  A large library product reaches 1.26.
 //
 // KR regions: 32-byte block u of row k sits at u ^ (2 (k & 3)): the 4 rows x 2 blocks that 32 lanes read together lie in all 64 banks once.
 #include "gated_linear.h"

@@ -5,20 +5,20 @@
 // Unlike the LSTM layers (lstm*.hip), whose recurrent product forces one step after the other, the map of a run of steps on the state is
 // affine, h -> A h + H, and two runs join as (A1, H1) then (A2, H2) = (A1 A2, A2 H1 + H2): time is parallel.
 //
-// A workgroup owns CL * VEC channels of one sequence (128 bytes of a row: whole cache lines) and walks its time in tiles of 128 steps (256 where
-// few workgroups have a short sequence, 32 or 64 where it is shorter): TL time lanes of L consecutive steps each, all of a tile's loads in flight at once and the next tile's
-// behind them.  Each lane folds its steps to (A, H) in registers, a wave joins its lanes by shuffles, the waves meet in LDS once per tile, and
-// every lane runs its steps again from registers with its true incoming state: each input is read from memory once.  What bounds it is HBM (4
-// tensors forward, 7 backward), with the two gates' exponentials and reciprocals close behind.  bf16, T 256, B 32, C 1024: 15.4 us forward (67 MB,
-// 4.4 TB/s), 25.4 us backward (117 MB, 4.6 TB/s), where a large copy reaches 5.0.
+// A workgroup owns CL * VEC channels of one sequence (128 bytes of a row where the device is full, 16 to 64 in the forms for small sizes) and walks its
+// time in tiles of 128 steps (256 where few workgroups have a short sequence, 32 or 64 where it is shorter): TL time lanes of L consecutive steps each,
+// all of a tile's loads in flight at once and the next tile's behind them.  Each lane folds its steps to (A, H) in registers, a wave joins its lanes by
+// shuffles, the waves meet in LDS once per tile, and every lane runs its steps again from registers with its true incoming state: each input is read from
+// memory once.  What bounds it is HBM (4 tensors forward, 7 backward), with the two gates' exponentials and reciprocals close behind.  bf16, T 256, B 32,
+// C 1024: 16.3 us forward (67 MB, 4.1 TB/s), 26.9 us backward (117 MB, 4.4 TB/s), where a large copy reaches 5.0.
 //
 // With few channels in flight (B * C small) and a long sequence the tiles of one sequence are spread over S workgroups ("spans"): a first
 // launch folds every span to (A, H), and the second joins the spans before its own, in order, in front of its first tile.
 //
 // Backward, with dh_t the gradient of h_t and e_t = a_t dh_t what reaches h_{t-1}:
 //     dh_t = dy_t s(o_t) + e_{t+1},   dv = (1 - a) dh,   df = dh (h_{t-1} - v) a (1 - a),   do = dy h s(o) (1 - s(o)),   dh_0 = e_1
-// e is the same kind of affine scan, run from the end with the same a.  The states are not kept but for one per tile (written by the forward
-// pass, 1/64 of a bf16 tensor at most): the backward tile runs its steps again.
+// e is the same kind of affine scan, run from the end with the same a.  The states are not kept but for one per tile, 4 bytes a channel (of a bf16 tensor
+// 1/64 at tiles of 128, 2 / T where T is one tile, written by the forward pass): the backward tile runs its steps again.
 //
 // All states, products and sums are float32; results are rounded once, at their store.  Time runs in processing order tau = 0 .. T-1,
 // t = tau or T-1-tau (reverse); a step at or past its sequence's length is the identity (A = 1, H = 0), is not loaded, and stores 0.
@@ -611,11 +611,12 @@ __global__ __launch_bounds__(256) void gated_recurrence_step_kernel(const T* f, 
 
 // How a size is cut, by the sizes alone (the states and the workspace go by it).  rows: groups of 64 channels of all sequences.
 //   tiles   128 steps, the last tile's loads beside this one's work; 256 by twice the threads for T 129 .. 512 while they leave the device half
-//           empty (T 256, B 1, C 1024: 6.3 us against 7.7 in float32, 7.2 against 8.4 in bf16); 32 or 64 for sequences no longer than that, whose
-//           other time lanes would idle (float32 T 8, B 300, C 512: 15.4 us against 46.9; T 64, B 64, C 1024: 16.8 against 24.0)
-//   spans   a lone workgroup takes 2.6 us a tile, 128 of them 3.2 TB/s; a second launch costs 5 us and half as many reads again at 4.6 TB/s.  So longer
-//           sequences are cut while rows < 128, into as many spans as make 1024 workgroups (T 1201, B 1, C 512 float32: 10.8 us against 28.7; T 4096,
-//           B 8, C 512: 73 against 90, bf16 42 against 96), and not beyond (T 1024, B 32, C 512, rows 256: 47.6 us whole against 73 cut)
+//           empty (T 256, B 4, C 1024 bf16: 5.9 us against 14.6; B 1: 4.6 against 5.0); 32 or 64 for sequences no longer than that, whose other time
+//           lanes would idle (float32 T 8, B 300, C 512: 15.1 us against 46.3; T 64, B 64, C 1024: 16.9 against 24.7)
+//   spans   a lone workgroup walks its tiles one after the other (T 32768, B 1, C 512 float32 forward: 339 us whole, 76 cut); a second launch costs 5 us
+//           and half as many reads again.  So longer sequences are cut while rows < 128, into as many spans as make 1024 workgroups (T 1201, B 1, C 512
+//           float32: 11.0 us against 16.8; T 4096, B 8, C 512: 73 against 146, bf16 45 against 156), and not beyond (T 1024, B 32, C 512 float32,
+//           rows 256: 47 us whole against 74 cut)
 struct RecPlan {
     int tile, S, span;
 };
@@ -655,12 +656,12 @@ int rec_launch(RecArgs p, const RecPlan& plan, hipStream_t s)
     return 0;
 }
 
-// Four channels a lane and 128 bytes of a row per workgroup where the device is full: 8 steps a lane in bf16 (fewer joins an element: 15.4 us against
-// 19.4 forward, 25.4 against 32 backward at T 256, B 32, C 1024), 4 in float32 (16 bytes a load: 16.3 against 21.0 forward, 25.4 against 29.2 backward
+// Four channels a lane and 128 bytes of a row per workgroup where the device is full: 8 steps a lane in bf16 (fewer joins an element: 17.4 us against
+// 23.8 forward, 27.8 against 34.3 backward at T 256, B 32, C 1024), 4 in float32 (16 bytes a load: 29.5 against 36.1 forward, 45.3 against 51.9 backward
 // at T 1201, B 7, C 333).  While all workgroups are resident at once, 8 waves a compute unit, the time is a lane's own chain, and less work a lane is
-// faster: one channel a lane (T 256, B 1, C 1024, forward / backward: float32 4.5 / 5.9 us against 6.2 / 9.0, bf16 4.4 / 5.7 against 7.1 / 10.4; past
-// that bound it loses: T 256, B 4 13.1 against 6.7), then, in bf16, half the steps (T 256, B 4: 5.7 / 8.2 against 7.4 / 11.0; T 256, B 15: 14.3
-// against 8.3).  Rows of fewer than four channels take one a lane always.
+// faster: one channel a lane (T 256, B 1, C 1024, forward / backward: float32 4.6 / 6.0 us against 6.4 / 9.9, bf16 4.6 / 6.0 against 7.6 / 11.3; past
+// that bound it loses: T 256, B 4 15.0 against 5.9), then, in bf16, half the steps (T 256, B 4: 5.9 / 8.6 against 7.9 / 12.0; past the bound, T 256, B 15:
+// 15.1 against 8.9).  Rows of fewer than four channels take one a lane always.  (Times of a call in a captured graph, both launches where it has two.)
 template <bool BWD, int TILE>
 int rec_dispatch_tile(const RecArgs& p, const RecPlan& plan, int dtype, hipStream_t s)
 {

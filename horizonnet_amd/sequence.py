@@ -38,7 +38,8 @@ def gated_recurrence(forget, value, out_gate=None, h0=None, lengths=None, direct
     the layout of a bidirectional LSTM's output.  lengths: int32 / int64 tensor ``[B]`` on the same device: a sequence's steps at or past its
     length are not read, their y (and gradients) are 0, and the state passes; values outside ``0 .. T`` count as the nearest bound.
 
-    y has the inputs' type; the state runs in float32 and h_last ``[B, C]`` is float32: the state behind the last step taken."""
+    y has the inputs' type; the state runs in float32 and h_last ``[B, C]`` is float32: the state behind the last step taken.  An infinite state stays
+    infinite until a gate of 0 (in bfloat16, one below 2**-126), which makes NaN of it as the formula does."""
     return (_native or _load()).gated_recurrence(forget, value, out_gate, h0, lengths, direction)
 
 
@@ -53,7 +54,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)`` in one kernel.  x ``[..., K]``, weights ``[F, K]`` (the layout of
     ``nn.Linear.weight``), biases ``[F]`` or None, each by itself; activation "silu", "gelu" (error function), "sigmoid" or "relu".  Products and
     activations run in float32 and the result ``[..., F]`` is rounded once to the inputs' type.  In bfloat16 the backward pass forms the
-    projections again and only the inputs stay in memory between the passes; in float32 (K >= 128) both projections are kept."""
+    projections again and only the inputs stay in memory between the passes; in float32 (K >= 128) both projections are kept.  The projections' gradients
+    are rounded to the inputs' type in front of the products for dx and the weights' gradients, which in bfloat16 makes those 1.4 times as far off as one
+    rounding would; the biases' gradients are sums of the unrounded ones."""
     return (_native or _load()).gated_linear(x, w_gate, w_up, b_gate, b_up, activation)
 
 
