@@ -44,6 +44,21 @@ def test_tracing_is_refused():
                 trace(lambda t: _calls(t)[k]())
 
 
+@torch.library.custom_op("horizonnet_tests::dropped", mutates_args=())
+def _dropped(x: torch.Tensor) -> torch.Tensor:
+    return hn.dropout(x, 0.5, 1)
+
+
+def test_registered_operators_may_be_traced():
+    """Inside the kernel of an operator that a program has registered, the trace records that operator: the call goes on (here to the missing device)."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(4, 2, 8)
+    for trace in (lambda fn: torch.jit.trace(fn, (x,), check_trace=False), lambda fn: make_fx(fn)(x)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            trace(lambda t: _dropped(t))
+
+
 def _fails(rc, text):
     assert rc != 0 and text in _lib.load().hn_last_error().decode()
 
