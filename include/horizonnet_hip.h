@@ -444,7 +444,7 @@ int hn_gated_recurrence_bwd(const void* f, int64_t f_t, int64_t f_b, const void*
                             int64_t o_b, const void* dy, int64_t dy_t, int64_t dy_b, const float* dh_last, const int* lengths,
                             const float* states, void* df, void* dv, void* d_o, float* dh0, float* workspace, size_t workspace_floats,
                             int64_t T, int64_t B, int64_t C, int dtype, int direction, void* stream);
-/* One step of B sequences: state [B][C] is updated in place, y [B][C]. */
+/* One step of B sequences: state [B][C] is updated in place, y [B][C].  f, v and o overlap the state nowhere or are it. */
 int hn_gated_recurrence_step(const void* f, int64_t f_b, const void* v, int64_t v_b, const void* o, int64_t o_b, float* state, void* y,
                              int64_t B, int64_t C, int dtype, void* stream);
 
