@@ -83,7 +83,7 @@ __device__ __forceinline__ float seq_exp(float x)
 
 // s(x) and 1 - s(x) = s(-x) from ONE exponential of -|x|: neither is formed by a subtraction from 1, so the small one keeps its relative
 // precision (a long memory is a small 1 - a).  Both are right to float32's last bits in both modes: the states that they make are float32, whatever the
-// type of the inputs (exponential 4 u, sum and reciprocal 3 u, product u).
+// type of the inputs (exponential 4 u, sum and reciprocal 2 u, product u).
 template <bool EXACT>
 __device__ __forceinline__ void seq_logistic(float x, float& s, float& rest)
 {

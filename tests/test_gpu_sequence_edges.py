@@ -43,8 +43,9 @@ def test_sigmoid_gate_saturated(name, M, K, F):
 
 def test_float32_results_of_bf16_recurrence():
     """The states and dh0 of a bf16 call are float32 and have to be right to float32's last bits: with v = 0 they are products of gates alone.  One
-    gate is off by 2 u for the exponential, u for the correction, u + 2 u for 1 + e and its reciprocal, u for the product: 7 u, and u more for the product
-    with the state; a second gate, of the output, adds as much again (the order in which steps are joined adds u a step)."""
+    gate is off by 2 u for the exponential, 0.9 u for what its constant leaves out, u for the sum that adds it, u for 1 + e, u for its reciprocal (in
+    [1/2, 1]) and u for the product: 6.9 u, and u more for the product with the state; a gate of the output in dh0 adds 6.9 u and the product u (the order in
+    which steps are joined adds u a step)."""
     u = ref.U
     g = torch.Generator().manual_seed(3)
     for T, B, C in ((1, 7, 130), (1, 300, 512), (2, 5, 64)):
